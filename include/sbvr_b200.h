@@ -397,6 +397,63 @@ SBVR_API int sbvr_ll_reduce_add_rmsnorm_digits_f16(const void* recv_local, const
                                                    int follows_push, int emit_digits, sbvr_workspace_t* ws,
                                                    sbvr_stream_t stream);
 
+/* ---- a KV cache in pages ----------------------------------------------------------------------------------------
+ * Sequences live in slots; a slot's tokens k * page .. lie in page table[slot][k] of every layer, and a page may belong to several slots that
+ * begin with the same tokens.  All pointers are device memory of the caller's; one call at a time may use a cache (they change it, and its
+ * scratch), calls on one stream are in order.  Device state decides what a call does (free pages, lengths), so it is found out on the device:
+ * what cannot be done leaves the cache as it was and a bit in *status, which stays until the caller clears it.  All calls are asynchronous and
+ * may be captured.  No counterpart in the reference, whose cache is the Hugging Face one (models/sbvr_llama.py:330-336). */
+typedef struct sbvr_pages {
+    void* pool;                         /* fp16 [layers][2: K, V][pages][n_kv][page][head_dim], 16-byte aligned */
+    int* table;                         /* [max_seqs][max_pages], -1 where a slot has no page */
+    int* lengths;                       /* [max_seqs] tokens that a slot holds */
+    int* refs;                          /* [pages rounded up to 4], 16-byte aligned: how many slots hold a page */
+    int* status;                        /* [1] SBVR_PAGES_* bits */
+    int* scratch;                       /* sbvr_pages_scratch_bytes(), 16-byte aligned */
+    int layers, pages, page;            /* page: tokens of a page, 16, 32, 64, 128 or 256 */
+    int n_kv, head_dim;                 /* head_dim 128 */
+    int max_seqs, max_pages;
+} sbvr_pages_t;
+enum {
+    SBVR_PAGES_NO_PAGE = 1,             /* fewer free pages than the call needs */
+    SBVR_PAGES_TOO_LONG = 2,            /* a slot would need more than max_pages */
+    SBVR_PAGES_BAD_SLOT = 4,            /* a slot out of range or named twice, a negative number of tokens */
+    SBVR_PAGES_NO_ENTRY = 8             /* a token was appended to, or read from, a place that the table names no page for: not stored, zeros */
+};
+SBVR_API int sbvr_pages_scratch_bytes(const sbvr_pages_t* cache, size_t* bytes);
+/* Room for tokens[i] (NULL: tokens_each) more tokens in slots[i] (NULL: slot i), n slots: the pages they lack, lowest free index first, the slots in
+ * order; lengths grow.  positions (may be NULL) [n][tokens_per_seq]: where the new tokens stand in their sequences, -1 behind the last. */
+SBVR_API int sbvr_pages_reserve(const sbvr_pages_t* cache, const int* slots, const int* tokens, int tokens_each, int n, int* positions,
+                                int tokens_per_seq, sbvr_stream_t stream);
+/* The slots hold nothing afterwards; a page that no other slot holds is free. */
+SBVR_API int sbvr_pages_free(const sbvr_pages_t* cache, const int* slots, int n, sbvr_stream_t stream);
+/* Slot dst[i] becomes what slot src[i] is before the call (at most 1024 pairs, all at once: a dst may be the src of another pair; src[i] == dst[i] changes
+ * nothing; no dst twice).  share = 1: whole pages are held in common, the tokens of a part-filled last page are copied to a page of the child's own.
+ * share = 0: all are copied.  New pages are the lowest that nobody holds once the children have given up theirs and that the call does not copy
+ * from. */
+SBVR_API int sbvr_pages_fork(const sbvr_pages_t* cache, const int* src, const int* dst, int n, int share, sbvr_stream_t stream);
+/* With U pages in use, moves those at U and behind, in order, to the free ones in front: afterwards pages 0 .. U - 1 are the ones in use. */
+SBVR_API int sbvr_pages_compact(const sbvr_pages_t* cache, sbvr_stream_t stream);
+/* shared[g] = tokens in front (whole pages) that the sequences group_starts[g] .. group_starts[g + 1] - 1 of a batch hold in the same pages; 0 for a
+ * group of one. */
+SBVR_API int sbvr_pages_common(const sbvr_pages_t* cache, const int* slots, int n, const int* group_starts, int groups, int* shared,
+                               sbvr_stream_t stream);
+/* As sbvr_rope_append_f16, to pages: q_out[token][n_heads * 128] = the rotated queries (zeros for a position below 0), k and v go to the pages of
+ * slots[token / tokens_per_seq] at positions[token] (below 0: nowhere).  qkv is left as it is.  Angles in 64 bits, the rotation in 32, one rounding. */
+SBVR_API int sbvr_pages_rope_append_f16(const sbvr_pages_t* cache, int layer, const void* qkv, const int* positions, const float* inv_freq,
+                                        float attn_scaling, const int* slots, int seqs, int tokens_per_seq, int n_heads, void* q_out,
+                                        sbvr_stream_t stream);
+/* out[token][head] = softmax(q . K^T * scale) . V over positions 0 .. positions[token] of the slot of sequence token / tokens_per_seq (none below 0:
+ * zeros).  q rows q_pitch elements apart (a multiple of 8), out [seqs * tokens_per_seq][n_heads * 128]; n_heads a multiple of n_kv; scale > 0.
+ * groups > 0: sequences group_starts[g] .. group_starts[g + 1] - 1 hold their first shared[g] tokens (whole pages count) in the same pages, those of
+ * the group's first sequence are read, once for all of them (sbvr_pages_common finds them); sequences in no group share nothing.  groups = 0: nothing is shared.
+ * scratch: sbvr_pages_attention_scratch_bytes(), 16-byte aligned, not used by another call at the same time. */
+SBVR_API int sbvr_pages_attention_scratch_bytes(const sbvr_pages_t* cache, int seqs, int tokens_per_seq, int n_heads, int groups, size_t* bytes);
+SBVR_API int sbvr_pages_attention_f16(const sbvr_pages_t* cache, int layer, const void* q, long long q_pitch, const int* slots,
+                                      const int* positions, const int* group_starts, const int* shared, int groups, void* out,
+                                      void* scratch, size_t scratch_bytes, int seqs, int tokens_per_seq, int n_heads, float scale,
+                                      sbvr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -368,6 +368,175 @@ PyObject* py_row_deq(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- a cache in pages (models/pages.py holds the tensors and the description of them) -----------------------------------------------
+// Every function begins (cache, device): the address of an sbvr_pages_t that the caller keeps, and the device of its memory.
+struct Pages {
+    const sbvr_pages_t* c;
+    int dev;
+    c10::cuda::OptionalCUDAGuard guard;
+    sbvr_stream_t stream;
+    Pages(PyObject* const* a, Py_ssize_t n, Py_ssize_t want, const char* name) {
+        if (n != want) fail(PyExc_TypeError, std::string(name) + " takes " + std::to_string(want) + " arguments");
+        c = reinterpret_cast<const sbvr_pages_t*>((uintptr_t)PyLong_AsUnsignedLongLong(a[0]));
+        dev = (int)PyLong_AsLong(a[1]);
+        if (PyErr_Occurred()) throw Raised();
+        if (c10::cuda::current_device() != dev) guard.set_index(dev);
+        stream = reinterpret_cast<sbvr_stream_t>(c10::cuda::getCurrentCUDAStream(dev).stream());
+    }
+    at::Device device() const { return at::Device(at::kCUDA, (c10::DeviceIndex)dev); }
+    // a contiguous tensor of the cache's device
+    at::Tensor tensor(PyObject* o, at::ScalarType type, const char* name) const {
+        at::Tensor t = opt_tensor(o, name);
+        if (!t.defined()) return t;
+        if (!t.is_cuda() || t.get_device() != dev) fail(PyExc_ValueError, std::string(name) + " must live on the cache's device");
+        if (t.scalar_type() != type) fail(PyExc_ValueError, std::string(name) + " must be " + at::toString(type));
+        if (!t.is_contiguous()) fail(PyExc_ValueError, std::string(name) + " must be contiguous");
+        return t;
+    }
+    at::Tensor need(PyObject* o, at::ScalarType type, const char* name) const {
+        at::Tensor t = tensor(o, type, name);
+        if (!t.defined()) fail(PyExc_TypeError, std::string(name) + " must be a tensor");
+        return t;
+    }
+    // slots of a batch; None: as many as `other` says, from slot 0 on
+    at::Tensor slots(PyObject* o, int64_t* n) const {
+        at::Tensor t = tensor(o, at::kInt, "slots");
+        if (t.defined()) *n = t.numel();
+        return t;
+    }
+};
+int as_int(PyObject* o) {
+    const long v = PyLong_AsLong(o);
+    if (v == -1 && PyErr_Occurred()) throw Raised();
+    if (v != (int)v) fail(PyExc_OverflowError, "argument does not fit 32 bits");
+    return (int)v;
+}
+const int* ints(const at::Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
+
+// pages_reserve(cache, device, slots, n, tokens (tensor or int), tokens_per_seq) -> positions or None
+PyObject* py_pages_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        c10::InferenceMode im;
+        Pages p(a, n, 6, "pages_reserve");
+        int64_t k = as_int(a[3]);
+        at::Tensor slots = p.slots(a[2], &k), tokens, positions;
+        const bool each = PyLong_Check(a[4]);
+        if (!each) {
+            tokens = p.need(a[4], at::kInt, "tokens");
+            if (tokens.numel() != k) fail(PyExc_ValueError, "tokens must name a number for every slot");
+        }
+        const int tps = as_int(a[5]);
+        if (tps < 0) fail(PyExc_ValueError, "tokens_per_seq must not be negative");
+        if (tps) positions = at::empty({k * tps}, at::TensorOptions().dtype(at::kInt).device(p.device()));
+        check(sbvr_pages_reserve(p.c, ints(slots), ints(tokens), each ? as_int(a[4]) : 0, (int)k, tps ? positions.data_ptr<int>() : nullptr, tps, p.stream),
+              "sbvr_pages_reserve");
+        if (!tps) Py_RETURN_NONE;
+        return THPVariable_Wrap(positions);
+    });
+}
+// pages_free(cache, device, slots)
+PyObject* py_pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Pages p(a, n, 3, "pages_free");
+        at::Tensor slots = p.need(a[2], at::kInt, "slots");
+        check(sbvr_pages_free(p.c, ints(slots), (int)slots.numel(), p.stream), "sbvr_pages_free");
+        Py_RETURN_NONE;
+    });
+}
+// pages_fork(cache, device, src, dst, share)
+PyObject* py_pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Pages p(a, n, 5, "pages_fork");
+        at::Tensor src = p.need(a[2], at::kInt, "src"), dst = p.need(a[3], at::kInt, "dst");
+        if (src.numel() != dst.numel()) fail(PyExc_ValueError, "src and dst must be of one length");
+        check(sbvr_pages_fork(p.c, ints(src), ints(dst), (int)src.numel(), as_int(a[4]), p.stream), "sbvr_pages_fork");
+        Py_RETURN_NONE;
+    });
+}
+// pages_compact(cache, device)
+PyObject* py_pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Pages p(a, n, 2, "pages_compact");
+        check(sbvr_pages_compact(p.c, p.stream), "sbvr_pages_compact");
+        Py_RETURN_NONE;
+    });
+}
+// pages_common(cache, device, slots, n, group_starts) -> shared
+PyObject* py_pages_common(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        c10::InferenceMode im;
+        Pages p(a, n, 5, "pages_common");
+        int64_t k = as_int(a[3]);
+        at::Tensor slots = p.slots(a[2], &k), starts = p.need(a[4], at::kInt, "group_starts");
+        const int64_t groups = starts.numel() - 1;
+        if (groups < 1) fail(PyExc_ValueError, "group_starts must hold one number more than there are groups");
+        at::Tensor out = at::empty({groups}, starts.options());
+        check(sbvr_pages_common(p.c, ints(slots), (int)k, ints(starts), (int)groups, out.data_ptr<int>(), p.stream), "sbvr_pages_common");
+        return THPVariable_Wrap(out);
+    });
+}
+// sequences of a batch and tokens of each, from the positions and the slots
+int64_t seqs_of(const Pages& p, const at::Tensor& slots, const at::Tensor& positions, int64_t all, int64_t* tps) {
+    const int64_t T = positions.numel(), n = slots.defined() ? slots.numel() : all;
+    if (T < 1 || n < 1 || T % n) fail(PyExc_ValueError, "positions must hold as many tokens for every sequence");
+    *tps = T / n;
+    return n;
+}
+// pages_rope_append(cache, device, layer, qkv, positions, inv_freq, scaling, slots, n, q_out) -> q
+PyObject* py_pages_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        c10::InferenceMode im;
+        Pages p(a, n, 10, "pages_rope_append");
+        at::Tensor qkv = p.need(a[3], at::kHalf, "qkv"), pos = p.need(a[4], at::kInt, "positions"), inv = p.need(a[5], at::kFloat, "inv_freq");
+        const double scaling = PyFloat_AsDouble(a[6]);
+        if (scaling == -1.0 && PyErr_Occurred()) throw Raised();
+        at::Tensor slots = p.tensor(a[7], at::kInt, "slots"), q = p.tensor(a[9], at::kHalf, "q_out");
+        int64_t tps;
+        const int64_t seqs = seqs_of(p, slots, pos, as_int(a[8]), &tps), T = pos.numel();
+        const int64_t D = p.c->head_dim, width = qkv.dim() ? qkv.size(-1) : 0, nh = width / D - 2 * p.c->n_kv;
+        if (qkv.dim() != 2 || qkv.size(0) != T || width % D || nh < 1) fail(PyExc_ValueError, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim]");
+        if (inv.numel() != D / 2) fail(PyExc_ValueError, "inv_freq must hold head_dim / 2 frequencies");
+        if (!q.defined()) q = empty_half({T, nh * D}, p.device());
+        else if (q.numel() != T * nh * D) fail(PyExc_ValueError, "q_out must be [tokens, n_heads * head_dim]");
+        check(sbvr_pages_rope_append_f16(p.c, as_int(a[2]), qkv.data_ptr(), ints(pos), inv.data_ptr<float>(), (float)scaling, ints(slots), (int)seqs, (int)tps,
+                                         (int)nh, q.data_ptr(), p.stream), "sbvr_pages_rope_append_f16");
+        return THPVariable_Wrap(q);
+    });
+}
+// pages_attention(cache, device, layer, q, positions, slots, n, scale, group_starts, shared, out) -> out
+PyObject* py_pages_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        c10::InferenceMode im;
+        Pages p(a, n, 11, "pages_attention");
+        at::Tensor q = opt_tensor(a[3], "q"), pos = p.need(a[4], at::kInt, "positions"), slots = p.tensor(a[5], at::kInt, "slots");
+        const double scale = PyFloat_AsDouble(a[7]);
+        if (scale == -1.0 && PyErr_Occurred()) throw Raised();
+        at::Tensor starts = p.tensor(a[8], at::kInt, "group_starts"), shared = p.tensor(a[9], at::kInt, "shared"), out = p.tensor(a[10], at::kHalf, "out");
+        int64_t tps;
+        const int64_t seqs = seqs_of(p, slots, pos, as_int(a[6]), &tps), T = pos.numel(), D = p.c->head_dim;
+        if (!q.defined() || !q.is_cuda() || q.get_device() != p.dev) fail(PyExc_ValueError, "q must live on the cache's device");
+        if (q.scalar_type() != at::kHalf) fail(PyExc_ValueError, "q must be Half");
+        if (q.dim() != 2 || q.size(0) != T || q.size(1) % D || q.stride(1) != 1) fail(PyExc_ValueError, "q must be [tokens, n_heads * head_dim], its rows contiguous");
+        const int64_t nh = q.size(1) / D;
+        int64_t groups = 0;
+        if (starts.defined() != shared.defined()) fail(PyExc_ValueError, "group_starts and shared go together");
+        if (starts.defined()) {
+            groups = shared.numel();
+            if (groups < 1 || starts.numel() != groups + 1) fail(PyExc_ValueError, "group_starts must hold one number more than shared");
+        }
+        if (!out.defined()) out = empty_half({T, nh * D}, p.device());
+        else if (out.numel() != T * nh * D) fail(PyExc_ValueError, "out must be [tokens, n_heads * head_dim]");
+        size_t bytes = 0;
+        check(sbvr_pages_attention_scratch_bytes(p.c, (int)seqs, (int)tps, (int)nh, (int)groups, &bytes), "sbvr_pages_attention_scratch_bytes");
+        at::Tensor scratch;                        // of this call: its memory goes to later work of the same stream (or graph) only
+        if (bytes) scratch = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(p.device()));
+        check(sbvr_pages_attention_f16(p.c, as_int(a[2]), q.data_ptr(), T > 1 ? q.stride(0) : nh * D, ints(slots), ints(pos), ints(starts), ints(shared), (int)groups,
+                                       out.data_ptr(), ptr(scratch), bytes, (int)seqs, (int)tps, (int)nh, (float)scale, p.stream),
+              "sbvr_pages_attention_f16");
+        return THPVariable_Wrap(out);
+    });
+}
+
 // set_workspace(device, stream, handle, nbytes): what `_lib.workspace` now holds for this pair
 PyObject* py_set_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -401,6 +570,15 @@ PyMethodDef g_methods[] = {
     {"decode", SBVR_FAST(py_decode), "decode(w) -> [N, K]"},
     {"mm_T", SBVR_FAST(py_mm_T), "mm_T(lhs, rhs, bias) -> [M, N] or None"},
     {"row_deq", SBVR_FAST(py_row_deq), "row_deq(x, bvr_t, idx, cache, bias) -> [M, N]"},
+    {"pages_reserve", SBVR_FAST(py_pages_reserve), "pages_reserve(cache, device, slots, n, tokens, tokens_per_seq) -> positions or None"},
+    {"pages_free", SBVR_FAST(py_pages_free), "pages_free(cache, device, slots)"},
+    {"pages_fork", SBVR_FAST(py_pages_fork), "pages_fork(cache, device, src, dst, share)"},
+    {"pages_compact", SBVR_FAST(py_pages_compact), "pages_compact(cache, device)"},
+    {"pages_common", SBVR_FAST(py_pages_common), "pages_common(cache, device, slots, n, group_starts) -> shared"},
+    {"pages_rope_append", SBVR_FAST(py_pages_rope_append),
+     "pages_rope_append(cache, device, layer, qkv, positions, inv_freq, scaling, slots, n, q_out) -> q"},
+    {"pages_attention", SBVR_FAST(py_pages_attention),
+     "pages_attention(cache, device, layer, q, positions, slots, n, scale, group_starts, shared, out) -> out"},
     {"set_workspace", SBVR_FAST(py_set_workspace), "set_workspace(device, stream, handle, nbytes)"},
     {"set_workspace_callback", SBVR_FAST(py_set_callback), "set_workspace_callback(f(device, stream, nbytes))"},
     {nullptr, nullptr, 0, nullptr}};

@@ -110,7 +110,31 @@ lib.sbvr_ll_reduce_add_rmsnorm_digits_f16.restype = _i
 lib.sbvr_allreduce_add_rmsnorm_digits_f16.argtypes = [_vp, _vp, _vp, _i, _i, _i, _i, _sz, _vp, _vp, _vp, _vp, _i, _i, _f, _i, _vp, _vp]
 lib.sbvr_allreduce_add_rmsnorm_digits_f16.restype = _i
 
-EXPORTS = ["sbvr_linear_folds", "sbvr_linear_workspace_bytes", "sbvr_linear_padded_f16", "sbvr_encode_stats_f16", "sbvr_encode_advance", "sbvr_encode_run", "sbvr_popc_mm_f16", "sbvr_linear_t_f16", "sbvr_encode_mse_f16", "sbvr_encode_select_f16", "sbvr_encode_pack", "sbvr_rope_attention_f16", "sbvr_linear_fused_f16", "sbvr_allreduce_add_rmsnorm_f16", "sbvr_linear_push_f16", "sbvr_ll_reduce_add_rmsnorm_f16", "sbvr_ll_reduce_add_rmsnorm_digits_f16", "sbvr_allreduce_add_rmsnorm_digits_f16", "sbvr_add_rmsnorm_f16", "sbvr_rope_append_f16", "sbvr_attention_f16", "sbvr_silu_mul_f16",
+
+
+class Pages(ctypes.Structure):
+    """sbvr_pages_t of include/sbvr_b200.h."""
+    _fields_ = ([(f, _vp) for f in ("pool", "table", "lengths", "refs", "status", "scratch")] +
+                [(f, _i) for f in ("layers", "pages", "page", "n_kv", "head_dim", "max_seqs", "max_pages")])
+
+
+PAGES_NO_PAGE, PAGES_TOO_LONG, PAGES_BAD_SLOT, PAGES_NO_ENTRY = 1, 2, 4, 8
+_pp = ctypes.POINTER(Pages)
+lib.sbvr_pages_scratch_bytes.argtypes = [_pp, ctypes.POINTER(_sz)]
+lib.sbvr_pages_reserve.argtypes = [_pp, _vp, _vp, _i, _i, _vp, _i, _vp]
+lib.sbvr_pages_free.argtypes = [_pp, _vp, _i, _vp]
+lib.sbvr_pages_fork.argtypes = [_pp, _vp, _vp, _i, _i, _vp]
+lib.sbvr_pages_compact.argtypes = [_pp, _vp]
+lib.sbvr_pages_common.argtypes = [_pp, _vp, _i, _vp, _i, _vp, _vp]
+lib.sbvr_pages_rope_append_f16.argtypes = [_pp, _i, _vp, _vp, _vp, _f, _vp, _i, _i, _i, _vp, _vp]
+lib.sbvr_pages_attention_scratch_bytes.argtypes = [_pp, _i, _i, _i, _i, ctypes.POINTER(_sz)]
+lib.sbvr_pages_attention_f16.argtypes = [_pp, _i, _vp, ctypes.c_longlong, _vp, _vp, _vp, _vp, _i, _vp, _vp, _sz, _i, _i, _i, _f, _vp]
+_PAGES = ["sbvr_pages_scratch_bytes", "sbvr_pages_reserve", "sbvr_pages_free", "sbvr_pages_fork", "sbvr_pages_compact", "sbvr_pages_common",
+          "sbvr_pages_rope_append_f16", "sbvr_pages_attention_scratch_bytes", "sbvr_pages_attention_f16"]
+for _name in _PAGES:
+    getattr(lib, _name).restype = _i
+
+EXPORTS = _PAGES + ["sbvr_linear_folds", "sbvr_linear_workspace_bytes", "sbvr_linear_padded_f16", "sbvr_encode_stats_f16", "sbvr_encode_advance", "sbvr_encode_run", "sbvr_popc_mm_f16", "sbvr_linear_t_f16", "sbvr_encode_mse_f16", "sbvr_encode_select_f16", "sbvr_encode_pack", "sbvr_rope_attention_f16", "sbvr_linear_fused_f16", "sbvr_allreduce_add_rmsnorm_f16", "sbvr_linear_push_f16", "sbvr_ll_reduce_add_rmsnorm_f16", "sbvr_ll_reduce_add_rmsnorm_digits_f16", "sbvr_allreduce_add_rmsnorm_digits_f16", "sbvr_add_rmsnorm_f16", "sbvr_rope_append_f16", "sbvr_attention_f16", "sbvr_silu_mul_f16",
            "sbvr_embedding_f16", "sbvr_argmax_f16", "sbvr_linear_f16_noalloc", "sbvr_workspace_bytes", "sbvr_strerror", "sbvr_last_cuda_error", "sbvr_last_timeout_where", "sbvr_last_timeout_info", "sbvr_query", "sbvr_workspace_create",
            "sbvr_workspace_destroy", "sbvr_workspace_status", "sbvr_workspace_patience", "sbvr_decode_f16", "sbvr_linear_f16",
            "sbvr_linear_f16_host"]

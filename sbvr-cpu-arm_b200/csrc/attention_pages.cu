@@ -8,66 +8,18 @@
 //
 // A part of a softmax is (m, l, o): o = sum of 2^(s - m) v, l = sum of 2^(s - m) over its keys, s the scores times scale * log2(e), all fp32.
 // Parts join as M = max m, l = sum l 2^(m - M), o = sum o 2^(m - M); a part without keys has m = -inf, l = 0.
-#include <cuda.h>
-
 #include <algorithm>
 #include <climits>
 
-#include "common.cuh"
-#include "pages.cuh"
-#include "tc_stream.cuh"
+#include "attention_pages.cuh"
 
 namespace sbvr {
-
-constexpr int AO_D = PG_D;
-// Weights become fp16 for the second product: half a step, 2^-11, of each.  They are multiplied by 2^10 first, so that what is 2^-24 and more of
-// the largest keeps all of its bits; the reference a weight is taken from may lag 2^5 behind the largest: at most 2^15.
-constexpr float AO_LIFT = 10.0f;
-
-struct AoParams {
-    PgCache c;
-    const __half* k;                               // this layer's planes
-    const __half* v;
-    const __half* q;
-    const int* slots;
-    const int* positions;
-    const int* starts;                             // [groups + 1], NULL: nothing is shared
-    const int* shared;                             // [groups]
-    __half* out;
-    float* part;                                   // [slots of parts][rows][130]
-    long long q_pitch;
-    int seqs, tps, n_heads, R, groups;
-    float sl2;                                     // scale * log2(e)
-    int per_block;                                 // sequences whose rows share a block
-    int ctas;                                      // shares of the first kernel
-};
-
-__device__ __forceinline__ float ao_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ int ao_slot(const AoParams& p, int seq) {
-    const int s = p.slots ? __ldg(p.slots + seq) : seq;
-    return s >= 0 && s < p.c.max_seqs ? s : -1;
-}
-// tokens that a row of a position attends to: none below zero, no more than a slot can hold
-__device__ __forceinline__ int ao_limit(const AoParams& p, int position) { return max(0, min(position + 1, p.c.max_pages * p.c.page)); }
-// the page of tokens k * page .. of a slot, -1 where the table names none
-__device__ __forceinline__ int ao_page(const AoParams& p, int slot, int k) {
-    const int e = slot >= 0 ? __ldg(p.c.table + (size_t)slot * p.c.max_pages + k) : -1;
-    return e >= 0 && e < p.c.pages ? e : -1;
-}
-__device__ __forceinline__ int ao_shared(const AoParams& p, int g) {
-    const int s = max(0, min(__ldg(p.shared + g), p.c.max_pages * p.c.page));
-    return s & ~(p.c.page - 1);
-}
 
 // ---------------------------------------------------------------------------------------------
 // A sequence's own keys.  A cluster of `nsplit` CTAs per (sequence, KV head, 16 rows); every warp takes sixteen keys at a time, a running maximum
 // and sums of its own: no barrier until the end, when the warps' and the CTAs' parts are joined through (distributed) shared memory.
 // ---------------------------------------------------------------------------------------------
-constexpr int AO_STAGES = 3, AO_KEYS = 16, AO_WARPS = 4;
+constexpr int AO_STAGES = 3, AO_KEYS = 16, AO_WARPS = 4, AO_PITCH = AO_D + 4;
 constexpr int AO_HALF_STAGE = AO_KEYS * AO_D * 2;                            // bytes of K or V of sixteen keys
 constexpr int AO_SMEM = AO_WARPS * AO_STAGES * 2 * AO_HALF_STAGE;            // 96 KB; later the warps' sums
 
@@ -101,6 +53,32 @@ __device__ __forceinline__ float2 ao_ld_cluster2(uint32_t a) {
     return v;
 }
 
+struct AoJoin {                                    // four dims of a row; `top` is found first
+    float top = -INFINITY, l = 0.0f;
+    float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    template <typename F>
+    __device__ __forceinline__ void add(const float2& ml, F&& value) {
+        const float f = ml.x == -INFINITY ? (ml.y != ml.y ? 1.0f : 0.0f) : ao_exp2(ml.x - top);        // (no keys; all of its scores are NaN)
+        if (f == 0.0f) return;
+        const float4 v = value();
+        o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+        l += f * ml.y;
+    }
+};
+__device__ __forceinline__ float2 ao_part_ml(const float* part, int rows, int row) {
+    return *reinterpret_cast<const float2*>(part + (size_t)rows * AO_D + (size_t)row * 2);
+}
+__device__ __forceinline__ float4 ao_part_o(const float* part, int rows, int row, int d4) {
+    return *reinterpret_cast<const float4*>(part + ((size_t)d4 * rows + row) * 4);
+}
+__device__ __forceinline__ void ao_put(const AoParams& p, int token, int head, int d4, const AoJoin& j) {
+    const float inv = 1.0f / j.l;
+    const bool on = j.l > 0.0f || j.l != j.l;      // (a row without keys: zeros)
+    const __half2 a = __floats2half2_rn(on ? j.o.x * inv : 0.0f, on ? j.o.y * inv : 0.0f), b = __floats2half2_rn(on ? j.o.z * inv : 0.0f, on ? j.o.w * inv : 0.0f);
+    *reinterpret_cast<uint2*>(p.out + ((size_t)token * p.n_heads + head) * AO_D + d4 * 4) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
 __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoParams p, int nsplit) {
     extern __shared__ __align__(128) unsigned char ao_smem[];
     __shared__ float2 ml_s[AO_WARPS][16];          // a warp's m, l
@@ -110,8 +88,16 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     const int unit = (int)blockIdx.x / nsplit, rank = (int)blockIdx.x - unit * nsplit;
     const int rb = unit % nrb, kvh = (unit / nrb) % p.c.n_kv, seq = unit / (nrb * p.c.n_kv);
     const int row0 = rb * 16, nrows = min(16, rps - row0);
+    // Behind the first kernel this one starts when that one's CTAs have all begun, which they do when everything in front of them has ended: only
+    // the parts are waited for, and last.
     pdl_launch_dependents();
-    pdl_wait();
+    const bool behind = p.starts != nullptr;
+    if (!behind) pdl_wait();
+    AoFind f = {};
+    long long total = 0;
+    f.g = -1;
+    if (behind) f = ao_find(p, 0, seq, &total);
+    const int from = f.g < 0 ? 0 : f.group.keys;   // tokens that the first kernel takes
     const int slot = ao_slot(p, seq);
     int lim[2];
     const __half* qrow[2];
@@ -123,6 +109,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     }
     const int most = __reduce_max_sync(0xffffffffu, max(lim[0], lim[1]));
     const int least = __reduce_min_sync(0xffffffffu, min(g < nrows ? lim[0] : INT_MAX, g + 8 < nrows ? lim[1] : INT_MAX));
+    const int seen = __reduce_min_sync(0xffffffffu, min(lim[0] > 0 ? lim[0] : INT_MAX, lim[1] > 0 ? lim[1] : INT_MAX));      // (rows without keys come out as zeros)
     uint32_t q[8][4];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -151,7 +138,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[16][4];
 #pragma unroll
     for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    int ch = rank * AO_WARPS + warp, stage = 0;
+    int ch = from / AO_KEYS + rank * AO_WARPS + warp, stage = 0;
 #pragma unroll
     for (int s = 0; s < AO_STAGES - 1; ++s) fetch(ch + s * step, s);
     for (; ch < chunks; ch += step) {
@@ -198,7 +185,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
 #pragma unroll
         for (int n = 0; n < 16; ++n) o[n][0] *= corr[0], o[n][1] *= corr[0], o[n][2] *= corr[1], o[n][3] *= corr[1];
         bool plain = true;
-        if (key0 + AO_KEYS > least && least < most) {              // a weight of zero hides finite values only
+        if (key0 + AO_KEYS > seen && seen < most) {              // a weight of zero hides finite values only
             uint32_t any = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -249,93 +236,136 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
     __syncthreads();                               // every warp is done with its ring
-    float* o_s = reinterpret_cast<float*>(ao_smem);                // [warp][16][128]
+    float* o_s = reinterpret_cast<float*>(ao_smem);                // [warp][16][AO_PITCH]
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (t4 == 0) ml_s[warp][g + 8 * h] = make_float2(m[h] == -INFINITY ? m[h] : m[h] - AO_LIFT, l[h]);
         if (g + 8 * h < nrows) {
 #pragma unroll
             for (int n = 0; n < 16; ++n)
-                *reinterpret_cast<float2*>(o_s + ((warp * 16 + g + 8 * h) * AO_D + n * 8 + 2 * t4)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                *reinterpret_cast<float2*>(o_s + ((warp * 16 + g + 8 * h) * AO_PITCH + n * 8 + 2 * t4)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         }
     }
     __syncthreads();
-    auto put = [&](int r, int d, const float4& v, float sum) {
-        const int row = row0 + r, tok = row / p.R;
-        const float inv = 1.0f / sum;
-        const bool on = sum > 0.0f || sum != sum;  // (a row without keys: zeros)
-        const __half2 a = __floats2half2_rn(on ? v.x * inv : 0.0f, on ? v.y * inv : 0.0f), b = __floats2half2_rn(on ? v.z * inv : 0.0f, on ? v.w * inv : 0.0f);
-        *reinterpret_cast<uint2*>(p.out + (((size_t)seq * p.tps + tok) * p.n_heads + (size_t)kvh * p.R + (row - tok * p.R)) * AO_D + d) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    };
     for (int it = tid; it < nrows * 32; it += AO_WARPS * 32) {     // four dims of a row
-        const int r = it >> 5, d = (it & 31) * 4;
-        float top = -INFINITY, sum = 0.0f;
+        const int r = it / 32, d = (it & 31) * 4;
+        AoJoin j;
 #pragma unroll
-        for (int w = 0; w < AO_WARPS; ++w) top = fmaxf(top, ml_s[w][r].x);
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (top != -INFINITY) {
+        for (int w = 0; w < AO_WARPS; ++w) j.top = fmaxf(j.top, ml_s[w][r].x);
 #pragma unroll
-            for (int w = 0; w < AO_WARPS; ++w) {
-                const float2 ml = ml_s[w][r];
-                const float f = ml.x == -INFINITY ? 0.0f : ao_exp2(ml.x - top);
-                if (f == 0.0f) continue;
-                const float4 v = *reinterpret_cast<const float4*>(o_s + (w * 16 + r) * AO_D + d);
-                acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-                sum += f * ml.y;
-            }
-        } else {
-#pragma unroll
-            for (int w = 0; w < AO_WARPS; ++w) sum += ml_s[w][r].y;                // (zero, or NaN where all scores are)
-            if (sum != sum) acc = make_float4(sum, sum, sum, sum);
-        }
-        if (nsplit == 1) {
-            put(r, d, acc, sum);
-        } else {
-            *reinterpret_cast<float4*>(o_s + r * AO_D + d) = acc;  // (warp 0's place, read by this thread)
-            if (d == 0) ml_c[r] = make_float2(top, sum);
-        }
+        for (int w = 0; w < AO_WARPS; ++w) j.add(ml_s[w][r], [&] { return *reinterpret_cast<const float4*>(o_s + (w * 16 + r) * AO_PITCH + d); });
+        *reinterpret_cast<float4*>(o_s + r * AO_PITCH + d) = j.o;  // (warp 0's place, read by this thread)
+        if (d == 0) ml_c[r] = make_float2(j.top, j.l);
     }
-    if (nsplit == 1) return;
-    ao_cluster_sync();
+    if (nsplit > 1) ao_cluster_sync();
+    else __syncthreads();
+    // ------------------------------ the parts of the CTAs and of the first kernel ------------------------------
+    if (behind) pdl_wait();
+    int c0 = 0, c1 = -1, seg = 0, prow = 0;
+    if (from > 0) {
+        const int shares = ao_shares(p, total), blk = (seq - f.group.s0) / p.per_block, in = kvh * f.group.blocks + blk;
+        const long long t0 = f.tile0 + (long long)in * f.group.tiles;
+        c0 = ao_share_of(total, shares, t0), c1 = ao_share_of(total, shares, t0 + f.group.tiles - 1);
+        seg = f.seg0 + in, prow = (seq - f.group.s0 - blk * p.per_block) * rps + row0;
+    }
     const uint32_t ob = smem_u32(o_s), mb = smem_u32(ml_c);
     for (int it = rank * AO_WARPS * 32 + tid; it < nrows * 32; it += nsplit * AO_WARPS * 32) {
-        const int r = it >> 5, d = (it & 31) * 4;
-        float top = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < nsplit; ++w) top = fmaxf(top, ao_ld_cluster2(ao_map_rank(mb + r * 8, w)).x);
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int w = 0; w < nsplit; ++w) {
-            const float2 ml = ao_ld_cluster2(ao_map_rank(mb + r * 8, w));
-            const float f = ml.x == -INFINITY ? (ml.y != ml.y ? 1.0f : 0.0f) : ao_exp2(ml.x - top);
-            if (f == 0.0f) continue;
-            const float4 v = ao_ld_cluster4(ao_map_rank(ob + (r * AO_D + d) * 4, w));
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-            sum += f * ml.y;
+        const int r = it % nrows, d4 = it / nrows;
+        const float* part = p.part + (size_t)(seg + c0) * ao_place_floats(p.rows);
+        AoJoin j;
+        for (int w = 0; w < nsplit; ++w) j.top = fmaxf(j.top, ao_ld_cluster2(ao_map_rank(mb + r * 8, w)).x);
+#pragma unroll 4
+        for (int c = 0; c <= c1 - c0; ++c) j.top = fmaxf(j.top, ao_part_ml(part + c * ao_place_floats(p.rows), p.rows, prow + r).x);
+        for (int w = 0; w < nsplit; ++w)
+            j.add(ao_ld_cluster2(ao_map_rank(mb + r * 8, w)), [&] { return ao_ld_cluster4(ao_map_rank(ob + (r * AO_PITCH + d4 * 4) * 4, w)); });
+#pragma unroll 4
+        for (int c = 0; c <= c1 - c0; ++c) {
+            const float* at = part + c * ao_place_floats(p.rows);
+            const float4 v = ao_part_o(at, p.rows, prow + r, d4);
+            j.add(ao_part_ml(at, p.rows, prow + r), [&] { return v; });
         }
-        put(r, d, acc, sum);
+        const int row = row0 + r, tok = row / p.R;
+        ao_put(p, seq * p.tps + tok, kvh * p.R + (row - tok * p.R), d4, j);
     }
-    ao_cluster_sync();                             // nobody leaves while its sums are read
+    if (nsplit > 1) ao_cluster_sync();             // nobody leaves while its sums are read
+}
+
+// ---------------------------------------------------------------------------------------------
+// The parts of a prompt's blocks, where several CTAs share a block's keys: 32 rows and four dims a warp.
+// ---------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) attention_join_kernel(const AoParams p, int nsplit) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int groups = p.rows / 32, block = (int)blockIdx.x / groups, row = ((int)blockIdx.x % groups) * 32 + (threadIdx.x & 31);
+    const int nblk = (p.tps * p.R + p.rows - 1) / p.rows, blk = block % nblk, u = block / nblk;
+    const int at_row = blk * p.rows + row, tok = at_row / p.R;
+    if (tok >= p.tps) return;
+    const int kvh = u % p.c.n_kv, seq = u / p.c.n_kv;
+    const float* part = p.part + (size_t)block * nsplit * ao_place_floats(p.rows);
+    for (int d4 = threadIdx.x >> 5; d4 < 32; d4 += 8) {
+        AoJoin j;
+        for (int c = 0; c < nsplit; ++c) j.top = fmaxf(j.top, ao_part_ml(part + c * ao_place_floats(p.rows), p.rows, row).x);
+#pragma unroll 4
+        for (int c = 0; c < nsplit; ++c) {
+            const float* at = part + c * ao_place_floats(p.rows);
+            const float4 v = ao_part_o(at, p.rows, row, d4);
+            j.add(ao_part_ml(at, p.rows, row), [&] { return v; });
+        }
+        ao_put(p, seq * p.tps + tok, kvh * p.R + (at_row - tok * p.R), d4, j);
+    }
 }
 
 }  // namespace sbvr
 
 using namespace sbvr;
 
-// CTAs that share the keys of a (sequence, KV head, 16 rows): as many as make about two per SM, at most 8
-static int own_split(int units, int sm_count) {
-    int n = 1;
-    while (n < 8 && units * n * 2 <= 2 * sm_count) n *= 2;
-    return n;
+// How a call is carried out.
+struct AoPlan {
+    bool prompt, shared;                           // rows of a sequence in blocks of their own; the first kernel runs
+    int rows, per_block, blocks, nsplit, ctas;     // blocks: of all sequences (prompt), at most (shared)
+    size_t places;                                 // of parts
+};
+static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int groups, int sm_count) {
+    AoPlan r = {};
+    const long long rps = (long long)tps * (n_heads / c.n_kv);
+    r.prompt = rps >= 64;
+    if (r.prompt) {
+        r.rows = rps > 128 ? 256 : 128;
+        r.blocks = (int)(seqs * c.n_kv * ((rps + r.rows - 1) / r.rows));
+        r.ctas = r.rows == 128 ? 2 * sm_count : sm_count;
+        r.nsplit = std::max(1, std::min(64, r.ctas / r.blocks));
+        r.places = r.nsplit > 1 ? (size_t)r.blocks * r.nsplit : 0;
+    } else {
+        r.shared = groups > 0;
+        if (r.shared) {
+            r.rows = seqs * rps > 128LL * groups ? 256 : 128;
+            r.per_block = r.rows / (int)rps;
+            r.ctas = r.rows == 128 ? 2 * sm_count : sm_count;
+            r.blocks = c.n_kv * (std::min(groups, seqs / 2) + seqs / r.per_block);     // (groups of two and more)
+            r.places = (size_t)r.blocks + r.ctas;
+        }
+        const long long units = (long long)seqs * c.n_kv * ((rps + 15) / 16);
+        r.nsplit = 1;                              // CTAs on a sequence's own keys: as many as make about two per SM, at most 8
+        while (r.nsplit < 8 && units * r.nsplit * 2 <= 2 * sm_count) r.nsplit *= 2;
+    }
+    return r;
 }
 
 extern "C" {
 
 int sbvr_pages_attention_scratch_bytes(const sbvr_pages_t* cache, int seqs, int tokens_per_seq, int n_heads, int groups, size_t* bytes) {
     PgCache c;
-    const int rc = pg_cache(cache, &c);
+    int rc = pg_cache(cache, &c);
     if (rc) return rc;
     if (!bytes || seqs < 1 || tokens_per_seq < 1 || n_heads < 1 || groups < 0 || n_heads % c.n_kv) return SBVR_ERR_BAD_ARG;
-    *bytes = 0;
+    if ((long long)seqs * tokens_per_seq > INT_MAX / 4 / n_heads) return SBVR_ERR_UNSUPPORTED;
+    DeviceInfo di;
+    int dev = 0;
+    SBVR_CUDA_TRY(cudaGetDevice(&dev));
+    rc = device_info(dev, &di);
+    if (rc) return rc;
+    const AoPlan r = ao_plan(c, seqs, tokens_per_seq, n_heads, groups, di.sm_count);
+    *bytes = r.places * ao_place_floats(r.rows) * sizeof(float);
     return SBVR_OK;
 }
 
@@ -350,26 +380,35 @@ int sbvr_pages_attention_f16(const sbvr_pages_t* cache, int layer, const void* q
         groups > seqs || (groups && (!group_starts || !shared)) || q_pitch < (long long)n_heads * AO_D || !(scale > 0.0f) || scale > 1e30f)
         return SBVR_ERR_BAD_ARG;
     if (!slots && seqs > c.max_seqs) return SBVR_ERR_BAD_ARG;
-    if ((long long)seqs * tokens_per_seq * n_heads > INT_MAX / 4) return SBVR_ERR_UNSUPPORTED;
-    if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) || q_pitch % 8) return SBVR_ERR_ALIGN;
+    if ((long long)seqs * tokens_per_seq > INT_MAX / 4 / n_heads) return SBVR_ERR_UNSUPPORTED;
+    if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) & 15) || q_pitch % 8) return SBVR_ERR_ALIGN;
     DeviceInfo di;
     int dev = 0;
     SBVR_CUDA_TRY(cudaGetDevice(&dev));
     rc = device_info(dev, &di);
     if (rc) return rc;
+    const AoPlan r = ao_plan(c, seqs, tokens_per_seq, n_heads, groups, di.sm_count);
+    if (r.places && (!scratch || scratch_bytes < r.places * ao_place_floats(r.rows) * sizeof(float))) return SBVR_ERR_WORKSPACE;
     p.k = c.pool + (size_t)layer * 2 * pg_plane(c), p.v = p.k + pg_plane(c);
-    p.q = static_cast<const __half*>(q), p.slots = slots, p.positions = positions, p.starts = groups ? group_starts : nullptr, p.shared = shared;
+    p.q = static_cast<const __half*>(q), p.slots = slots, p.positions = positions, p.starts = r.shared ? group_starts : nullptr, p.shared = shared;
     p.out = static_cast<__half*>(out), p.part = static_cast<float*>(scratch), p.q_pitch = q_pitch;
-    p.seqs = seqs, p.tps = tokens_per_seq, p.n_heads = n_heads, p.R = n_heads / c.n_kv, p.groups = groups;
+    p.seqs = seqs, p.tps = tokens_per_seq, p.n_heads = n_heads, p.R = n_heads / c.n_kv, p.groups = r.shared ? groups : 0;
     p.sl2 = scale * 1.4426950408889634f;
-    (void)scratch_bytes;
+    p.rows = r.rows, p.per_block = r.per_block, p.ctas = r.ctas;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    static SmemOnce once, once_cluster;
+    if (r.prompt || r.shared) {
+        rc = launch_attention_shared(p, r.prompt, r.nsplit, r.prompt ? r.blocks * r.nsplit : r.ctas, st);
+        if (rc) return rc;
+    }
+    if (r.prompt) {
+        if (r.nsplit > 1) SBVR_CUDA_TRY(launch_pdl(attention_join_kernel, dim3((unsigned)(r.blocks * (r.rows / 32))), dim3(256), 0, st, p, r.nsplit));
+        return SBVR_OK;
+    }
+    static SmemOnce once;
     rc = set_max_smem_once(once, attention_own_kernel, AO_SMEM);
-    if (!rc) rc = set_attribute_once(once_cluster, attention_own_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (rc) return rc;
-    const int units = seqs * c.n_kv * ((p.tps * p.R + 15) / 16), nsplit = own_split(units, di.sm_count);
-    SBVR_CUDA_TRY(launch_pdl_cluster(attention_own_kernel, dim3((unsigned)(units * nsplit)), dim3(AO_WARPS * 32), nsplit, (size_t)AO_SMEM, st, p, nsplit));
+    const int units = seqs * c.n_kv * ((p.tps * p.R + 15) / 16);
+    SBVR_CUDA_TRY(launch_pdl_cluster(attention_own_kernel, dim3((unsigned)(units * r.nsplit)), dim3(AO_WARPS * 32), r.nsplit, (size_t)AO_SMEM, st, p, r.nsplit));
     return SBVR_OK;
 }
 

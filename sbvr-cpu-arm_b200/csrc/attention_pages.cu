@@ -19,9 +19,9 @@ namespace sbvr {
 // A sequence's own keys.  A cluster of `nsplit` CTAs per (sequence, KV head, 16 rows); every warp takes sixteen keys at a time, a running maximum
 // and sums of its own: no barrier until the end, when the warps' and the CTAs' parts are joined through (distributed) shared memory.
 // ---------------------------------------------------------------------------------------------
-constexpr int AO_STAGES = 3, AO_KEYS = 16, AO_WARPS = 4, AO_PITCH = AO_D + 4;
+constexpr int AO_STAGES = 2, AO_KEYS = 16, AO_WARPS = 4, AO_PITCH = AO_D + 4;
 constexpr int AO_HALF_STAGE = AO_KEYS * AO_D * 2;                            // bytes of K or V of sixteen keys
-constexpr int AO_SMEM = AO_WARPS * AO_STAGES * 2 * AO_HALF_STAGE;            // 96 KB; later the warps' sums
+constexpr int AO_SMEM = AO_WARPS * AO_STAGES * 2 * AO_HALF_STAGE;            // 64 KB; later the warps' sums
 
 __device__ __forceinline__ void ao_ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -53,16 +53,25 @@ __device__ __forceinline__ float2 ao_ld_cluster2(uint32_t a) {
     return v;
 }
 
-struct AoJoin {                                    // four dims of a row; `top` is found first
+struct AoJoin {                                    // four dims of a row: parts joined as they come
     float top = -INFINITY, l = 0.0f;
     float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    template <typename F>
-    __device__ __forceinline__ void add(const float2& ml, F&& value) {
-        const float f = ml.x == -INFINITY ? (ml.y != ml.y ? 1.0f : 0.0f) : ao_exp2(ml.x - top);        // (no keys; all of its scores are NaN)
-        if (f == 0.0f) return;
-        const float4 v = value();
-        o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
-        l += f * ml.y;
+    // N parts whose values are in registers (no keys: m = -inf, l = 0; m = -inf and l = NaN: all scores are)
+    template <int N>
+    __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&v)[N]) {
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < N; ++i) now = fmaxf(now, ml[i].x);
+        const float c = top == -INFINITY ? (l != l ? 1.0f : 0.0f) : ao_exp2(top - now);
+        top = now;
+        o.x *= c, o.y *= c, o.z *= c, o.w *= c, l *= c;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float f = ml[i].x == -INFINITY ? (ml[i].y != ml[i].y ? 1.0f : 0.0f) : ao_exp2(ml[i].x - top);
+            if (f == 0.0f) continue;               // (what lies there may be anything)
+            o.x += f * v[i].x, o.y += f * v[i].y, o.z += f * v[i].z, o.w += f * v[i].w;
+            l += f * ml[i].y;
+        }
     }
 };
 __device__ __forceinline__ float2 ao_part_ml(const float* part, int rows, int row) {
@@ -70,6 +79,23 @@ __device__ __forceinline__ float2 ao_part_ml(const float* part, int rows, int ro
 }
 __device__ __forceinline__ float4 ao_part_o(const float* part, int rows, int row, int d4) {
     return *reinterpret_cast<const float4*>(part + ((size_t)d4 * rows + row) * 4);
+}
+// n parts of a row, eight at a time on their way
+__device__ __forceinline__ void ao_join_parts(AoJoin& j, const float* part, int n, int rows, int row, int d4) {
+    for (int c0 = 0; c0 < n; c0 += 8) {
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float* at = part + (size_t)min(c0 + c, n - 1) * ao_place_floats(rows);
+            ml[c] = ao_part_ml(at, rows, row);
+            v[c] = ao_part_o(at, rows, row, d4);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c0 + c >= n) ml[c] = make_float2(-INFINITY, 0.0f);
+        j.add(ml, v);
+    }
 }
 __device__ __forceinline__ void ao_put(const AoParams& p, int token, int head, int d4, const AoJoin& j) {
     const float inv = 1.0f / j.l;
@@ -93,11 +119,6 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     pdl_launch_dependents();
     const bool behind = p.starts != nullptr;
     if (!behind) pdl_wait();
-    AoFind f = {};
-    long long total = 0;
-    f.g = -1;
-    if (behind) f = ao_find(p, 0, seq, &total);
-    const int from = f.g < 0 ? 0 : f.group.keys;   // tokens that the first kernel takes
     const int slot = ao_slot(p, seq);
     int lim[2];
     const __half* qrow[2];
@@ -116,6 +137,11 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
         q[k][0] = *reinterpret_cast<const uint32_t*>(qrow[0] + k * 16 + 2 * t4), q[k][1] = *reinterpret_cast<const uint32_t*>(qrow[1] + k * 16 + 2 * t4);
         q[k][2] = *reinterpret_cast<const uint32_t*>(qrow[0] + k * 16 + 8 + 2 * t4), q[k][3] = *reinterpret_cast<const uint32_t*>(qrow[1] + k * 16 + 8 + 2 * t4);
     }
+    AoPiece f = {};
+    f.g = -1;
+    if (behind) f = ao_find(p, ao_density(p), -1, seq);
+    const int blk = f.g < 0 ? 0 : (seq - f.group.s0) / p.per_block, place = f.piece0 + (kvh * f.group.blocks + blk) * f.n;
+    const int from = f.g < 0 || place + f.n > p.places ? 0 : f.group.keys;     // tokens that the first kernel takes
     const int step = nsplit * AO_WARPS, chunks = (most + AO_KEYS - 1) / AO_KEYS;
     const uint32_t ring = smem_u32(ao_smem) + warp * (AO_STAGES * 2 * AO_HALF_STAGE);
     auto fetch = [&](int ch, int stage) {          // sixteen keys lie in one page
@@ -250,10 +276,11 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     for (int it = tid; it < nrows * 32; it += AO_WARPS * 32) {     // four dims of a row
         const int r = it / 32, d = (it & 31) * 4;
         AoJoin j;
+        float2 ml[AO_WARPS];
+        float4 v[AO_WARPS];
 #pragma unroll
-        for (int w = 0; w < AO_WARPS; ++w) j.top = fmaxf(j.top, ml_s[w][r].x);
-#pragma unroll
-        for (int w = 0; w < AO_WARPS; ++w) j.add(ml_s[w][r], [&] { return *reinterpret_cast<const float4*>(o_s + (w * 16 + r) * AO_PITCH + d); });
+        for (int w = 0; w < AO_WARPS; ++w) ml[w] = ml_s[w][r], v[w] = *reinterpret_cast<const float4*>(o_s + (w * 16 + r) * AO_PITCH + d);
+        j.add(ml, v);
         *reinterpret_cast<float4*>(o_s + r * AO_PITCH + d) = j.o;  // (warp 0's place, read by this thread)
         if (d == 0) ml_c[r] = make_float2(j.top, j.l);
     }
@@ -261,29 +288,24 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     else __syncthreads();
     // ------------------------------ the parts of the CTAs and of the first kernel ------------------------------
     if (behind) pdl_wait();
-    int c0 = 0, c1 = -1, seg = 0, prow = 0;
-    if (from > 0) {
-        const int shares = ao_shares(p, total), blk = (seq - f.group.s0) / p.per_block, in = kvh * f.group.blocks + blk;
-        const long long t0 = f.tile0 + (long long)in * f.group.tiles;
-        c0 = ao_share_of(total, shares, t0), c1 = ao_share_of(total, shares, t0 + f.group.tiles - 1);
-        seg = f.seg0 + in, prow = (seq - f.group.s0 - blk * p.per_block) * rps + row0;
-    }
+    const int prow = (seq - f.group.s0 - blk * p.per_block) * rps + row0;
+    const float* part = p.part + (size_t)place * ao_place_floats(p.rows);
     const uint32_t ob = smem_u32(o_s), mb = smem_u32(ml_c);
     for (int it = rank * AO_WARPS * 32 + tid; it < nrows * 32; it += nsplit * AO_WARPS * 32) {
         const int r = it % nrows, d4 = it / nrows;
-        const float* part = p.part + (size_t)(seg + c0) * ao_place_floats(p.rows);
         AoJoin j;
-        for (int w = 0; w < nsplit; ++w) j.top = fmaxf(j.top, ao_ld_cluster2(ao_map_rank(mb + r * 8, w)).x);
-#pragma unroll 4
-        for (int c = 0; c <= c1 - c0; ++c) j.top = fmaxf(j.top, ao_part_ml(part + c * ao_place_floats(p.rows), p.rows, prow + r).x);
-        for (int w = 0; w < nsplit; ++w)
-            j.add(ao_ld_cluster2(ao_map_rank(mb + r * 8, w)), [&] { return ao_ld_cluster4(ao_map_rank(ob + (r * AO_PITCH + d4 * 4) * 4, w)); });
-#pragma unroll 4
-        for (int c = 0; c <= c1 - c0; ++c) {
-            const float* at = part + c * ao_place_floats(p.rows);
-            const float4 v = ao_part_o(at, p.rows, prow + r, d4);
-            j.add(ao_part_ml(at, p.rows, prow + r), [&] { return v; });
+        for (int w0 = 0; w0 < nsplit; w0 += 4) {
+            float2 ml[4];
+            float4 v[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int c = min(w0 + w, nsplit - 1);
+                ml[w] = ao_ld_cluster2(ao_map_rank(mb + r * 8, c)), v[w] = ao_ld_cluster4(ao_map_rank(ob + (r * AO_PITCH + d4 * 4) * 4, c));
+                if (w0 + w >= nsplit) ml[w] = make_float2(-INFINITY, 0.0f);
+            }
+            j.add(ml, v);
         }
+        if (from > 0) ao_join_parts(j, part, f.n, p.rows, prow + r, d4);
         const int row = row0 + r, tok = row / p.R;
         ao_put(p, seq * p.tps + tok, kvh * p.R + (row - tok * p.R), d4, j);
     }
@@ -304,13 +326,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AoParams p, i
     const float* part = p.part + (size_t)block * nsplit * ao_place_floats(p.rows);
     for (int d4 = threadIdx.x >> 5; d4 < 32; d4 += 8) {
         AoJoin j;
-        for (int c = 0; c < nsplit; ++c) j.top = fmaxf(j.top, ao_part_ml(part + c * ao_place_floats(p.rows), p.rows, row).x);
-#pragma unroll 4
-        for (int c = 0; c < nsplit; ++c) {
-            const float* at = part + c * ao_place_floats(p.rows);
-            const float4 v = ao_part_o(at, p.rows, row, d4);
-            j.add(ao_part_ml(at, p.rows, row), [&] { return v; });
-        }
+        ao_join_parts(j, part, nsplit, p.rows, row, d4);
         ao_put(p, seq * p.tps + tok, kvh * p.R + (at_row - tok * p.R), d4, j);
     }
 }
@@ -336,13 +352,15 @@ static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int grou
         r.nsplit = std::max(1, std::min(64, r.ctas / r.blocks));
         r.places = r.nsplit > 1 ? (size_t)r.blocks * r.nsplit : 0;
     } else {
-        r.shared = groups > 0;
+        // What sharing can save at most: reading what the slots can hold once per group instead of once per sequence.  Below 2 MB the second kernel alone is
+        // the faster form: it reads that in the time that the first takes to begin.
+        r.shared = groups > 0 && (long long)(seqs - groups) * c.max_pages * c.page * c.n_kv * (4 * AO_D) > (2 << 20);
         if (r.shared) {
             r.rows = seqs * rps > 128LL * groups ? 256 : 128;
             r.per_block = r.rows / (int)rps;
             r.ctas = r.rows == 128 ? 2 * sm_count : sm_count;
             r.blocks = c.n_kv * (std::min(groups, seqs / 2) + seqs / r.per_block);     // (groups of two and more)
-            r.places = (size_t)r.blocks + r.ctas;
+            r.places = (size_t)r.blocks + AS_ROUNDS * r.ctas;  // (ao_density)
         }
         const long long units = (long long)seqs * c.n_kv * ((rps + 15) / 16);
         r.nsplit = 1;                              // CTAs on a sequence's own keys: as many as make about two per SM, at most 8
@@ -394,7 +412,7 @@ int sbvr_pages_attention_f16(const sbvr_pages_t* cache, int layer, const void* q
     p.out = static_cast<__half*>(out), p.part = static_cast<float*>(scratch), p.q_pitch = q_pitch;
     p.seqs = seqs, p.tps = tokens_per_seq, p.n_heads = n_heads, p.R = n_heads / c.n_kv, p.groups = r.shared ? groups : 0;
     p.sl2 = scale * 1.4426950408889634f;
-    p.rows = r.rows, p.per_block = r.per_block, p.ctas = r.ctas;
+    p.rows = r.rows, p.per_block = r.per_block, p.ctas = r.ctas, p.places = (int)std::min<size_t>(r.places, INT_MAX);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (r.prompt || r.shared) {
         rc = launch_attention_shared(p, r.prompt, r.nsplit, r.prompt ? r.blocks * r.nsplit : r.ctas, st);

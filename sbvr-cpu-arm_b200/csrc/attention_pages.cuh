@@ -2,6 +2,8 @@
 // into equal shares (attention_pages.cu, attention_shared.cu).
 #pragma once
 
+#include <climits>
+
 #include "common.cuh"
 #include "pages.cuh"
 
@@ -27,7 +29,7 @@ struct AoParams {
     int seqs, tps, n_heads, R, groups;
     float sl2;                                     // scale * log2(e)
     int rows, per_block;                           // first kernel: rows of a block, sequences whose rows share one
-    int ctas;                                      // ... CTAs, shares of the keys at most
+    int ctas, places;                              // ... CTAs of a round, parts there is room for
 };
 
 __device__ __forceinline__ float ao_exp2(float x) {
@@ -69,57 +71,85 @@ __device__ __forceinline__ AoGroup ao_group(const AoParams& p, int g) {
     r.tiles = (r.keys + AS_KEYS - 1) / AS_KEYS;
     return r;
 }
-// All tiles in order: groups, KV heads, blocks, tiles.  `find` looks for a tile (x) or for the group of a sequence (seq >= 0), a warp together.
-struct AoFind {
+// Every block's tiles are cut evenly into pieces, as many per block as its share of the tiles is of `rounds` times the CTAs: one round unless another
+// number of them ends sooner by AS_EXTRA, what a piece costs on top of its own tiles (queries, the first keys, sums).  A warp works it out together, a lane
+// per group; all of this runs once per CTA on a cold instruction cache, so it is kept short (a search for the longest piece, in 64 bits, took 4 us).
+constexpr int AS_EXTRA = 6, AS_ROUNDS = 3;
+struct AoPiece {
     AoGroup group;
     int g;                                         // -1: there is none
-    long long tile0;                               // first tile of the group
-    int seg0;                                      // first (KV head, block) of the group
+    int n;                                         // pieces of a block
+    int piece0;                                    // first piece of the group: its KV heads, blocks, pieces
 };
-__device__ __forceinline__ long long ao_warp_add(long long v, int lane) {      // inclusive prefix sums
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += y;
-    }
-    return v;
+__device__ __forceinline__ AoGroup ao_lane_group(const AoParams& p, int base) {
+    AoGroup r = {};
+    if (base + (int)(threadIdx.x & 31) < p.groups) r = ao_group(p, base + (threadIdx.x & 31));
+    return r;
 }
-__device__ __forceinline__ AoFind ao_find(const AoParams& p, long long x, int seq, long long* total) {
-    const int lane = threadIdx.x & 31;
-    AoFind f = {};
-    f.g = -1;
-    long long tiles = 0;
-    int segs = 0;
+// pieces of a block, for `density` pieces per tile
+__device__ __forceinline__ int ao_pieces(const AoGroup& g, float density) {
+    return max(1, min((int)(g.tiles * density), (g.tiles + AS_LEAST - 1) / AS_LEAST));
+}
+__device__ __forceinline__ float ao_density(const AoParams& p) {
+    float tiles = 0.0f;
     for (int base = 0; base < p.groups; base += 32) {
-        AoGroup gr = {};
-        if (base + lane < p.groups) gr = ao_group(p, base + lane);
-        const int segs_of = gr.blocks * p.c.n_kv;
-        const long long mine = (long long)segs_of * gr.tiles;
-        const long long up = ao_warp_add(mine, lane), sup = ao_warp_add(segs_of, lane);
-        const bool hit = base + lane < p.groups && (seq >= 0 ? gr.s0 <= seq && seq < gr.s1 : tiles + up - mine <= x && x < tiles + up);
-        const unsigned int any = __ballot_sync(0xffffffffu, hit);
-        if (any && f.g < 0) {
+        const AoGroup g = ao_lane_group(p, base);
+        tiles += (float)g.tiles * (float)(g.blocks * p.c.n_kv);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    const float one = (float)p.ctas / fmaxf(tiles, 1.0f);
+    int pieces[AS_ROUNDS] = {}, most[AS_ROUNDS] = {};
+    for (int base = 0; base < p.groups; base += 32) {
+        const AoGroup g = ao_lane_group(p, base);
+#pragma unroll
+        for (int r = 0; r < AS_ROUNDS; ++r) {
+            const int n = ao_pieces(g, one * (r + 1));
+            pieces[r] += n * g.blocks * p.c.n_kv;
+            most[r] = max(most[r], (g.tiles + n - 1) / n);
+        }
+    }
+    int best = INT_MAX, rounds = 1;
+#pragma unroll
+    for (int r = 0; r < AS_ROUNDS; ++r) {
+        const int sum = (int)__reduce_add_sync(0xffffffffu, (unsigned int)pieces[r]), top = __reduce_max_sync(0xffffffffu, most[r]);
+        const int cost = (sum + p.ctas - 1) / p.ctas * (top + AS_EXTRA);
+        if (cost < best) best = cost, rounds = r + 1;
+    }
+    return one * rounds;
+}
+// the group of a piece, or (piece < 0) of a sequence
+__device__ __forceinline__ AoPiece ao_find(const AoParams& p, float density, int piece, int seq) {
+    const int lane = threadIdx.x & 31;
+    AoPiece f = {};
+    f.g = -1;
+    int sum = 0;
+#pragma unroll 1
+    for (int base = 0; base < p.groups && f.g < 0; base += 32) {
+        const AoGroup gr = ao_lane_group(p, base);
+        const int n = ao_pieces(gr, density), mine = n * gr.blocks * p.c.n_kv;
+        int up = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += y;
+        }
+        up += sum;
+        const unsigned int any = __ballot_sync(0xffffffffu, piece >= 0 ? up - mine <= piece && piece < up : gr.s0 <= seq && seq < gr.s1);
+        if (any) {
             const int l = __ffs(any) - 1;
             f.g = base + l;
             f.group.s0 = __shfl_sync(0xffffffffu, gr.s0, l), f.group.s1 = __shfl_sync(0xffffffffu, gr.s1, l);
             f.group.keys = __shfl_sync(0xffffffffu, gr.keys, l);
             f.group.blocks = __shfl_sync(0xffffffffu, gr.blocks, l), f.group.tiles = __shfl_sync(0xffffffffu, gr.tiles, l);
-            f.tile0 = tiles + __shfl_sync(0xffffffffu, up - mine, l);
-            f.seg0 = segs + (int)__shfl_sync(0xffffffffu, sup - segs_of, l);
+            f.n = __shfl_sync(0xffffffffu, n, l), f.piece0 = __shfl_sync(0xffffffffu, up - mine, l);
         }
-        tiles += __shfl_sync(0xffffffffu, up, 31);
-        segs += (int)__shfl_sync(0xffffffffu, sup, 31);
+        sum = __shfl_sync(0xffffffffu, up, 31);
     }
-    *total = tiles;
     return f;
 }
-// CTAs that share `total` tiles, the first tile of one of them, and the CTA of a tile
-__device__ __forceinline__ int ao_shares(const AoParams& p, long long total) { return (int)max(1LL, min((long long)p.ctas, total / AS_LEAST)); }
-__device__ __forceinline__ long long ao_first(long long total, int shares, int c) { return total * c / shares; }
-__device__ __forceinline__ int ao_share_of(long long total, int shares, long long x) { return (int)(((x + 1) * shares - 1) / total); }
 
-// The part that share c leaves of block `seg`: segments and shares only grow along the tiles, so their sum names a place of its own.
-// [place]: O [32 fours of dims][rows][4], then (m, l) [rows][2]
+// The part that a piece leaves: O [32 fours of dims][rows][4], then (m, l) [rows][2].
 __host__ __device__ inline size_t ao_place_floats(int rows) { return (size_t)rows * (AO_D + 2); }
 
 // prompt: nsplit CTAs per block of a sequence's rows, else `grid` CTAs on what groups share

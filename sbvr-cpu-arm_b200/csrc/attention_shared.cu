@@ -16,6 +16,8 @@
 // rows out without the tensor cores.
 #include <cuda.h>
 
+#include <climits>
+
 #include "attention_pages.cuh"
 #include "attention_tc.cuh"
 #include "tc_stream.cuh"
@@ -23,7 +25,7 @@
 namespace sbvr {
 
 constexpr uint32_t AS_QBOX = 128 * 128, AS_KBOX = AS_KEYS * 128, AS_TILE = 2 * AS_KBOX;        // boxes of 64 dims, a tile of K or V
-constexpr int AS_HDR = 3072;
+constexpr int AS_HDR = 1024;
 
 template <int NT>
 struct AsShape {
@@ -33,26 +35,135 @@ struct AsShape {
     static constexpr uint32_t COLS = 256 * NT;
 };
 
-struct AsSeg {                                     // what a CTA works on at a time
-    int seq0, seq1;                                // sequences whose rows it has (prompt: one)
-    int row0;                                      // prompt: first row of the sequence
+__device__ __forceinline__ float as_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float2 as_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 as_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// the largest of 32 scores
+__device__ __forceinline__ float as_top32(const uint32_t* u) {
+    float m[4] = {__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]), __uint_as_float(u[3])};
+#pragma unroll
+    for (int e = 4; e < 32; e += 2) m[(e >> 1) & 3] = as_max3(m[(e >> 1) & 3], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+    return as_max3(fmaxf(m[0], m[1]), m[2], m[3]);
+}
+// sixteen columns of tensor memory
+__device__ __forceinline__ void aq_st16(uint32_t taddr, const uint32_t* a) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(a[0]), "r"(a[1]),
+                 "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]), "r"(a[8]), "r"(a[9]), "r"(a[10]), "r"(a[11]), "r"(a[12]), "r"(a[13]),
+                 "r"(a[14]), "r"(a[15])
+                 : "memory");
+}
+// 2^x of two numbers by multiplications and additions: the whole part by the exponent, the rest, at most a half, by a polynomial of degree 4 fitted to the
+// smallest largest relative error (2.7e-6, a 180th of fp16's half step).  Below 2^-125 it stays at that; NaN stays NaN.
+__device__ __forceinline__ float2 as_exp2_pair(float2 x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.0f));
+    const float2 big = make_float2(12582912.0f, 12582912.0f);           // 1.5 * 2^23: rounds to a whole number
+    const float2 t = as_add2(x, big), n = as_add2(t, make_float2(-12582912.0f, -12582912.0f)), f = as_fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 y = as_fma2(make_float2(9.570101276040077e-3f, 9.570101276040077e-3f), f, make_float2(5.591785907745361e-2f, 5.591785907745361e-2f));
+    y = as_fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    y = as_fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    y = as_fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    const float2 s = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+    return as_fma2(y, s, make_float2(0.0f, 0.0f));
+}
+// weights 2^(s sl2 - base) of 32 scores as fp16, their sums added to `sum`.  AS_POLY of sixteen pairs go the way above, which leaves the units for
+// exponentials (4 lanes a cycle and scheduler) that many fewer.
+constexpr int AS_POLY = 0;
+__device__ __forceinline__ void as_weights32(const uint32_t* u, float sl2, float base, uint32_t* w, float2 (&sum)[2]) {
+    const float2 a = make_float2(sl2, sl2), c = make_float2(-base, -base);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        float2 x = as_fma2(make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])), a, c);
+        if ((e * AS_POLY) % 16 + AS_POLY > 15) x = as_exp2_pair(x);
+        else x.x = ao_exp2(x.x), x.y = ao_exp2(x.y);
+        sum[e & 1] = as_add2(sum[e & 1], x);
+        const __half2 h = __floats2half2_rn(x.x, x.y);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+struct AsSeg {                                     // a piece: what a CTA works on at a time
+    int tok0, ntok;                                // tokens whose rows it has
+    int row0, rows;                                // its first row among those of the first token, rows
     int kvh, slot;                                 // slot whose table is read
     int ta, tb;                                    // tiles
-    int keys;                                      // 0: as many as its rows attend to (prompt)
+    int keys;                                      // keys that any row attends to
+    int least;                                     // ... that all rows do (which attend to any)
     int place;                                     // of its part, -1: the output
 };
 
-// row i of the block -> token, query head; false where there is none
-__device__ __forceinline__ bool as_row(const AoParams& p, const AsSeg& s, bool prompt, int i, int* token, int* head) {
-    const int rps = p.tps * p.R;
-    if (prompt) {
-        const int r = s.row0 + i, t = r / p.R;
-        *token = s.seq0 * p.tps + t, *head = s.kvh * p.R + (r - t * p.R);
-        return t < p.tps;
+// row i of a piece -> token, query head
+__device__ __forceinline__ void as_row(const AoParams& p, const AsSeg& s, int i, int* token, int* head) {
+    const int r = s.row0 + i, t = r / p.R;
+    *token = s.tok0 + t, *head = s.kvh * p.R + (r - t * p.R);
+}
+// keys that row i attends to, -1 where there is no such row
+template <bool PROMPT>
+__device__ __forceinline__ int as_limit(const AoParams& p, const AsSeg& s, int i) {
+    if (i >= s.rows) return -1;
+    const int lim = ao_limit(p, __ldg(p.positions + s.tok0 + (s.row0 + i) / p.R));
+    return PROMPT ? lim : min(lim, s.keys);
+}
+
+// piece number `j` of this CTA; false: there are no more.  Every warp finds out by itself.
+template <int ROWS, bool PROMPT>
+__device__ __forceinline__ bool as_piece(const AoParams& p, float density, int nsplit, int j, AsSeg& s) {
+    const int lane = threadIdx.x & 31;
+    if (PROMPT) {
+        if (j) return false;
+        const int rps = p.tps * p.R, nblk = (rps + ROWS - 1) / ROWS, per = p.seqs * p.c.n_kv, u = (int)blockIdx.x / nsplit;
+        const int blk = nblk - 1 - u / per, seq = u % per / p.c.n_kv;          // (the last rows have the longest contexts: first)
+        s.kvh = u % per % p.c.n_kv;
+        s.tok0 = seq * p.tps, s.row0 = blk * ROWS, s.rows = min(ROWS, rps - s.row0);
+        const int t0 = s.row0 / p.R;
+        s.tok0 += t0, s.row0 -= t0 * p.R;
+        s.slot = ao_slot(p, seq);
+        s.place = nsplit == 1 ? -1 : ((seq * p.c.n_kv + s.kvh) * nblk + blk) * nsplit + (int)blockIdx.x % nsplit;
+        s.keys = INT_MAX;
+    } else {
+        const int piece = (int)blockIdx.x + j * (int)gridDim.x;
+        if (piece >= p.places) return false;                     // (only where groups overlap)
+        const AoPiece f = ao_find(p, density, piece, -1);
+        if (f.g < 0) return false;
+        const int in = piece - f.piece0, seg = in / f.n, i = in - seg * f.n, each = f.group.tiles / f.n, more = f.group.tiles - each * f.n;
+        s.ta = each * i + min(i, more), s.tb = s.ta + each + (i < more ? 1 : 0);
+        s.kvh = seg / f.group.blocks;
+        const int seq = f.group.s0 + (seg - s.kvh * f.group.blocks) * p.per_block;
+        s.tok0 = seq * p.tps, s.row0 = 0, s.rows = min(p.per_block, f.group.s1 - seq) * p.tps * p.R;
+        s.slot = ao_slot(p, f.group.s0), s.keys = f.group.keys;
+        s.place = piece;
     }
-    const int q = i / rps, r = i - q * rps, t = r / p.R;
-    *token = (s.seq0 + q) * p.tps + t, *head = s.kvh * p.R + (r - t * p.R);
-    return s.seq0 + q < s.seq1;
+    s.ntok = (s.row0 + s.rows + p.R - 1) / p.R;
+    int hi = 0, lo = INT_MAX;
+    for (int t = lane; t < s.ntok; t += 32) {
+        const int lim = min(s.keys, ao_limit(p, __ldg(p.positions + s.tok0 + t)));
+        hi = max(hi, lim);
+        if (lim > 0) lo = min(lo, lim);
+    }
+    s.least = __reduce_min_sync(0xffffffffu, lo);
+    if (PROMPT) {
+        s.keys = __reduce_max_sync(0xffffffffu, hi);
+        const int tiles = (s.keys + AS_KEYS - 1) / AS_KEYS, per = max((tiles + nsplit - 1) / nsplit, nsplit > 1 ? AS_LEAST : 1);
+        s.ta = min(tiles, (int)blockIdx.x % nsplit * per), s.tb = min(tiles, s.ta + per);
+    }
+    return true;
 }
 
 __device__ __forceinline__ void as_store(const AoParams& p, int place, int rows, int row, int dim4, const float4& v) {
@@ -62,19 +173,20 @@ __device__ __forceinline__ void as_store_ml(const AoParams& p, int place, int ro
     *reinterpret_cast<float2*>(p.part + (size_t)place * ao_place_floats(rows) + (size_t)rows * AO_D + (size_t)row * 2) = make_float2(m, l);
 }
 
-// all rows of a block without the tensor cores: a warp each, four dims a lane, key by key
-__device__ __noinline__ void as_multiply_out(const AoParams& p, const AsSeg& s, bool prompt, int rows, const int* lim_s) {
+// all rows of a piece without the tensor cores: a warp each, four dims a lane, key by key
+template <bool PROMPT>
+__device__ __noinline__ void as_multiply_out(const AoParams& p, const AsSeg& s, int rows) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     auto four = [](const uint2& v, float (&f)[4]) {
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
         f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
     };
-    for (int row = warp; row < rows; row += warps) {
+    for (int row = warp; row < s.rows; row += warps) {
         int token, head;
-        if (!as_row(p, s, prompt, row, &token, &head)) continue;
+        as_row(p, s, row, &token, &head);
         float q[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
         four(*reinterpret_cast<const uint2*>(p.q + (size_t)token * p.q_pitch + (size_t)head * AO_D + lane * 4), q);
-        const int end = min(lim_s[row], s.tb * AS_KEYS);
+        const int end = min(as_limit<PROMPT>(p, s, row), s.tb * AS_KEYS);
         for (int key = s.ta * AS_KEYS; key < end; ++key) {
             const int page = ao_page(p, s.slot, key >> p.c.page_shift);
             float k[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -122,12 +234,10 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
     uint64_t* o_done = p_full + 2 * NT;                          // [NT][2] O has a tile's products
     uint64_t* drained = o_done + 2 * NT;                         // after a time-out
     uint64_t* landed = drained + 1;                              // a tile of V that is looked through before it is given out
+    uint64_t* q_full = landed + 1;                               // [NT] the queries of a piece are in shared memory
     volatile int* dead_s = reinterpret_cast<volatile int*>(smem + 384);
     uint32_t* tmem_s = reinterpret_cast<uint32_t*>(smem + 388);
-    volatile int* odd_s = reinterpret_cast<volatile int*>(smem + 392);
-    int* most_s = reinterpret_cast<int*>(smem + 396);            // keys that any row attends to, that every row (with keys) does, rows
-    int* least_s = most_s + 1;
-    int* lim_s = reinterpret_cast<int*>(smem + 512);             // [ROWS]
+    volatile int* odd_s = reinterpret_cast<volatile int*>(smem + 392);          // bit j % 32: piece j has to be multiplied out
     const uint32_t q_s = smem_u32(smem) + AS_HDR, k_s = q_s + NT * 2 * AS_QBOX, v_s = k_s + ST * AS_TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -141,6 +251,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
             mbar_init(o_done + i, 1);
         }
         mbar_init(drained, 1), mbar_init(landed, 1);
+        for (int i = 0; i < NT; ++i) mbar_init(q_full + i, 4);
         *dead_s = 0, *odd_s = 0;
         fence_mbar_init();
     }
@@ -156,83 +267,12 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
     __syncthreads();
     aq_fence_after();
     const uint32_t tbase = *tmem_s;
+    const float density = PROMPT ? 0.0f : ao_density(p);
     bool ok = true;
-    long long x = 0, x_end = 0, total = 0;                       // this CTA's tiles of the list
-    int shares = 1;
-    if (!PROMPT) {
-        ao_find(p, 0, -1, &total);
-        shares = ao_shares(p, total);
-        if ((int)blockIdx.x < shares) x = ao_first(total, shares, blockIdx.x), x_end = ao_first(total, shares, blockIdx.x + 1);
-    } else {
-        x_end = 1;
-    }
-    int looked = 0;                                              // tiles of V that were looked through
     int n0 = 0;                                                  // tiles that went through the rings so far
-    int m0[NT];                                                  // ... that a set of 128 rows has seen
-#pragma unroll
-    for (int i = 0; i < NT; ++i) m0[i] = 0;
+    AsSeg s;
 
-    while (x < x_end) {
-        // ------------------------------ the next block ------------------------------
-        AsSeg s;
-        if (PROMPT) {
-            const int nblk = (p.tps * p.R + ROWS - 1) / ROWS, part = (int)blockIdx.x % nsplit;
-            int u = (int)blockIdx.x / nsplit;
-            const int per = p.seqs * p.c.n_kv;
-            const int blk = nblk - 1 - u / per;                  // (the last rows have the longest contexts)
-            u %= per;
-            s.seq0 = u / p.c.n_kv, s.seq1 = s.seq0 + 1, s.kvh = u % p.c.n_kv, s.row0 = blk * ROWS;
-            s.slot = ao_slot(p, s.seq0);
-            s.ta = part, s.tb = 0, s.keys = 0;
-            s.place = nsplit == 1 ? -1 : ((s.seq0 * p.c.n_kv + s.kvh) * nblk + blk) * nsplit + part;
-            x = x_end;
-        } else {
-            long long t;
-            const AoFind f = ao_find(p, x, -1, &t);
-            const int in = (int)(x - f.tile0), seg = in / f.group.tiles;
-            s.ta = in - seg * f.group.tiles;
-            s.tb = (int)min((long long)f.group.tiles, s.ta + (x_end - x));
-            s.kvh = seg / f.group.blocks;
-            s.seq0 = f.group.s0 + (seg % f.group.blocks) * p.per_block, s.seq1 = min(f.group.s1, s.seq0 + p.per_block), s.row0 = 0;
-            s.slot = ao_slot(p, f.group.s0), s.keys = f.group.keys;
-            s.place = f.seg0 + seg + (int)blockIdx.x;
-            x += s.tb - s.ta;
-        }
-        if (threadIdx.x == 0) *most_s = 0, *least_s = 0x7fffffff, *odd_s = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < ROWS; i += W::THREADS) {
-            int token, head, lim = -1;                           // -1: no row
-            if (as_row(p, s, PROMPT, i, &token, &head)) {
-                lim = ao_limit(p, __ldg(p.positions + token));
-                if (!PROMPT) lim = min(lim, s.keys);
-            }
-            lim_s[i] = lim;
-            const int hi = __reduce_max_sync(0xffffffffu, lim), lo = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
-            if (lane == 0) atomicMax(most_s, hi), atomicMin(least_s, lo);
-        }
-        for (int c = threadIdx.x; c < ROWS * 16; c += W::THREADS) {
-            const int row = c >> 4, ch = c & 15;
-            int token, head;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (as_row(p, s, PROMPT, row, &token, &head)) v = *reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_pitch + (size_t)head * AO_D + ch * 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_s + (row >> 7) * 2 * AS_QBOX + (ch >> 3) * AS_QBOX + (row & 127) * 128 +
-                                                                       (((ch & 7) ^ (row & 7)) << 4)),
-                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                         : "memory");
-        }
-        fence_proxy_async();                                     // the MMAs read through the asynchronous proxy
-        __syncthreads();
-        const int P = PROMPT ? max(*most_s, 0) : s.keys, pmin = *least_s;
-        if (PROMPT) {
-            const int tiles = (P + AS_KEYS - 1) / AS_KEYS, per = max((tiles + nsplit - 1) / nsplit, nsplit > 1 ? AS_LEAST : 1);
-            const int part = s.ta;
-            s.ta = min(tiles, part * per), s.tb = min(tiles, s.ta + per);
-        }
-        const int cnt = s.tb - s.ta;
-        const int sets = NT == 1 || lim_s[NT == 1 ? 0 : 128] < 0 ? 1 : 2;      // sets of 128 rows that hold any
-
-        if (*dead_s) {                                           // (a wait ran out before: the rest without the tensor cores)
-        } else if (warp == W::KWARP || warp == W::VWARP) {
+    if (warp == W::KWARP || warp == W::VWARP) {
             // ------------------------------ K, V ------------------------------
             const bool is_k = warp == W::KWARP;
             uint64_t* empty = is_k ? k_empty : v_empty;
@@ -241,7 +281,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
             const uint32_t box_bytes = AS_KBOX / boxes;
             auto entry = [&](int t) {                            // row of the map where this lane's box of tile t begins
                 const int key = t * AS_KEYS + (lane << sh);
-                if (lane >= boxes || t >= s.tb || key >= P) return nowhere;
+                if (lane >= boxes || t >= s.tb || key >= s.keys) return nowhere;
                 const int page = ao_page(p, s.slot, key >> sh);
                 if (page < 0) {
                     atomicOr(p.c.status, SBVR_PAGES_NO_ENTRY);
@@ -249,16 +289,18 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                 }
                 return (page * p.c.n_kv + s.kvh) * p.c.page + (key & (p.c.page - 1));
             };
-            int y = entry(s.ta);
-            for (int i = 0; i < cnt; ++i) {
-                const int n = n0 + i, b = n % ST, next = entry(s.ta + i + 1);
-                if (n >= ST && (*dead_s || !mbar_wait_async(empty + b, (uint32_t)(n / ST - 1) & 1u))) ok = false;
+            int looked = 0;                                      // tiles of V that were looked through
+            for (int j = 0; ok && as_piece<ROWS, PROMPT>(p, density, nsplit, j, s); ++j) {
+              int y = entry(s.ta);
+              for (int t = s.ta; t < s.tb; ++t, ++n0) {
+                const int b = n0 % ST, next = entry(t + 1);
+                if (n0 >= ST && (*dead_s || !mbar_wait_async(empty + b, (uint32_t)(n0 / ST - 1) & 1u))) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 unsigned char* dst = smem + AS_HDR + NT * 2 * AS_QBOX + ((is_k ? 0 : ST) + b) * AS_TILE;
                 // Keys that not every row attends to: a weight of zero hides finite values only.  Behind the last key zeros take the place of
                 // whatever lies there; in front of it the CTA leaves the tensor cores where a value is not finite.
-                const bool look = !is_k && (s.ta + i + 1) * AS_KEYS > pmin;
+                const bool look = !is_k && (t + 1) * AS_KEYS > s.least;
                 uint64_t* bar = look ? landed : full + b;
                 if (lane == 0) mbar_arrive_expect_tx(bar, AS_TILE);
                 __syncwarp();
@@ -273,7 +315,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                     ++looked;
                     ok = __all_sync(0xffffffffu, there);
                     if (!ok) break;
-                    const int last = P - (s.ta + i) * AS_KEYS;   // rows of the tile from here on: nobody's
+                    const int last = s.keys - t * AS_KEYS;   // rows of the tile from here on: nobody's
 #pragma unroll 4
                     for (int e = lane; e < (int)AS_TILE / 16; e += 32) {
                         const uint32_t at = v_s + b * AS_TILE + e * 16;
@@ -284,45 +326,51 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                         uint32_t v[4];
                         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) any |= (v[j] & 0x7c007c00u) + 0x04000400u;     // (an exponent of all ones: bit 15)
+                        for (int e4 = 0; e4 < 4; ++e4) any |= (v[e4] & 0x7c007c00u) + 0x04000400u;     // (an exponent of all ones: bit 15)
                     }
-                    if (any & 0x80008000u) *odd_s = 1;
+                    if (any & 0x80008000u) atomicOr(const_cast<int*>(odd_s), 1 << (j & 31));
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full + b);
                 }
                 y = next;
+              }
             }
             if (!ok) *dead_s = 1;
         } else if (warp == W::IWARP) {
             // ------------------------------ MMA issuer ------------------------------
-            if (elect_one()) {
+            int m0[NT], j0[NT];                                  // tiles and pieces that a set of 128 rows has seen
+#pragma unroll
+            for (int r = 0; r < NT; ++r) m0[r] = j0[r] = 0;
+            for (int j = 0; ok && as_piece<ROWS, PROMPT>(p, density, nsplit, j, s); ++j) {
+              const int cnt = s.tb - s.ta, sets = NT == 2 && s.rows > 128 ? 2 : 1;
+              if (elect_one()) {
                 constexpr uint32_t QK = (1u << 4) | ((AS_KEYS >> 3) << 17) | ((128 >> 4) << 24);
                 constexpr uint32_t PV = (1u << 4) | (1u << 16) | ((AO_D >> 3) << 17) | ((128 >> 4) << 24);     // (bit 16: B is V as it lies)
                 const uint32_t qd = (q_s >> 4) | (1u << 16), kd = (k_s >> 4) | (1u << 16), vd = (v_s >> 4) | ((AS_KBOX >> 4) << 16);
-                auto scores = [&](int i) {
-                    const int n = n0 + i, b = n % ST;
-                    if (*dead_s || !mbar_wait_async(k_full + b, (uint32_t)(n / ST) & 1u)) return false;
+                auto scores = [&](int r, int i) {                // S of a set of rows: two tiles ahead of its weights
+                    const int n = n0 + i, b = n % ST, sb = (m0[r] + i) & 1;
+                    if (r == 0 && (*dead_s || !mbar_wait_async(k_full + b, (uint32_t)(n / ST) & 1u))) return false;
                     aq_fence_after();
 #pragma unroll
-                    for (int r = 0; r < NT; ++r) {
-                        if (r >= sets) break;
-                        const int sb = (m0[r] + i) & 1;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            aq_mma_ss(tbase + r * 256 + sb * 64, qd + r * (2 * AS_QBOX >> 4) + (k >> 2) * (AS_QBOX >> 4) + (k & 3) * 2,
-                                      kd + b * (AS_TILE >> 4) + (k >> 2) * (AS_KBOX >> 4) + (k & 3) * 2, QK, k ? 1u : 0u);
-                        aq_commit(s_full + 2 * r + sb);
-                    }
-                    aq_commit(k_empty + b);
+                    for (int k = 0; k < 8; ++k)
+                        aq_mma_ss(tbase + r * 256 + sb * 64, qd + r * (2 * AS_QBOX >> 4) + (k >> 2) * (AS_QBOX >> 4) + (k & 3) * 2,
+                                  kd + b * (AS_TILE >> 4) + (k >> 2) * (AS_KBOX >> 4) + (k & 3) * 2, QK, k ? 1u : 0u);
+                    aq_commit(s_full + 2 * r + sb);
+                    if (r == sets - 1) aq_commit(k_empty + b);
                     return true;
                 };
-                if (cnt) ok = scores(0);
+#pragma unroll
+                for (int r = 0; r < NT; ++r)
+                    if (r < sets && ok && (*dead_s || !mbar_wait_async(q_full + r, (uint32_t)j0[r] & 1u))) ok = false;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < NT; ++r)
+                        if (r < sets && i < cnt && ok) ok = scores(r, i);
                 for (int i = 0; i < cnt && ok; ++i) {
                     const int n = n0 + i, b = n % ST;
-                    // (S of the tile after the next lies over the weights of this one: their MMAs are in front of it)
-                    if (i + 1 < cnt && !scores(i + 1)) ok = false;
-                    if (ok && !mbar_wait_async(v_full + b, (uint32_t)(n / ST) & 1u)) ok = false;
+                    if (!mbar_wait_async(v_full + b, (uint32_t)(n / ST) & 1u)) ok = false;
 #pragma unroll
                     for (int r = 0; r < NT; ++r) {
                         if (r >= sets || !ok) break;
@@ -334,8 +382,9 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                         for (int k = 0; k < 4; ++k)              // sixteen keys: 2 KB of V, eight columns of weights
                             aq_mma_ts(tbase + r * 256 + 128, tbase + r * 256 + sb * 64 + k * 8, vd + b * (AS_TILE >> 4) + k * 128, PV, (i | k) ? 1u : 0u);
                         aq_commit(o_done + 2 * r + sb);
+                        if (r == sets - 1) aq_commit(v_empty + b);
+                        if (i + 2 < cnt) ok = scores(r, i + 2);  // (over the weights of this tile: their MMAs are in front of it)
                     }
-                    if (ok) aq_commit(v_empty + b);
                 }
                 if (!ok) {                                       // MMAs that were issued end before the CTA goes on
                     *dead_s = 1;
@@ -343,77 +392,119 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                     aq_commit(drained);
                     while (!mbar_test(drained, 0u) && clock64() - c0 < 200000000LL) {}
                 }
+              }
+              ok = __all_sync(0xffffffffu, ok);
+              n0 += cnt;
+#pragma unroll
+              for (int r = 0; r < NT; ++r)
+                  if (r < sets) m0[r] += cnt, ++j0[r];
             }
-            __syncwarp();
-        } else if ((warp >> 2) < sets) {
+        } else {
             // ------------------------------ weights ------------------------------
             const int r = warp >> 2, row = warp * 32 + lane;     // (row of the block: 128 r + 32 (warp % 4) + lane)
-            const int lim = lim_s[row];
+            const uint32_t mine = tbase + r * 256 + ((uint32_t)((warp & 3) * 32) << 16);
+            int mr = 0;                                          // tiles that these 128 rows have seen
+            for (int j = 0; as_piece<ROWS, PROMPT>(p, density, nsplit, j, s); ++j) {
+            const int cnt = s.tb - s.ta;
+            if (r && s.rows <= 128) continue;                    // (a piece without rows for this set)
+            // The queries of the warp's rows (the scores of the piece before are formed: its output was waited for).
+            int token = 0, head = 0;
+            const bool here = row < s.rows;
+            if (here) as_row(p, s, row, &token, &head);
+            {
+                const long long from = here ? (long long)token * p.q_pitch + (long long)head * AO_D : -1;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const int q = 2 * c + (lane >> 4), ch = lane & 15;
+                    const long long at = __shfl_sync(0xffffffffu, from, q);
+                    const uint32_t dst = q_s + r * 2 * AS_QBOX + (ch >> 3) * AS_QBOX + ((warp & 3) * 32 + q) * 128 + (((ch & 7) ^ (q & 7)) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p.q + (at < 0 ? 0 : at) + ch * 8), "r"(at < 0 ? 0u : 16u) : "memory");
+                }
+            }
+            const int lim = as_limit<PROMPT>(p, s, row);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async();                                 // the MMAs read through the asynchronous proxy
+            aq_fence_before();                                   // (and what was read of the piece before has been)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + r);
             const int wmin = __reduce_min_sync(0xffffffffu, lim < 0 ? 0x7fffffff : lim);        // (no rows: anything finite)
             const bool idle = !__any_sync(0xffffffffu, lim > 0);
-            const uint32_t mine = tbase + r * 256 + ((uint32_t)((warp & 3) * 32) << 16);
-            int mr = 0;
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-                if (i == r) mr = m0[i];
             const float sl2 = p.sl2;
+            // Half a tile at a time, the next half on its way.  Weights are formed with the reference there is, and once more where a score turns out too
+            // large for it: nothing waits for the largest score.  References are whole numbers (of scores times sl2), so that what was formed with the
+            // last one is scaled by a power of two.
             float ref = -INFINITY, sum = 0.0f;
+            uint32_t u[2][32], w[2][16];
+            bool ahead = false;                                  // the first half is on its way
             for (int i = 0; i < cnt; ++i) {
-                const int m = mr + i, b = m & 1;
-                if (*dead_s || !mbar_wait_async(s_full + 2 * r + b, (uint32_t)(m >> 1) & 1u)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                aq_fence_after();
+                const int m = mr + i, b = m & 1, key0 = (s.ta + i) * AS_KEYS;
+                if (!ahead) {
+                    if (*dead_s || !mbar_wait_async(s_full + 2 * r + b, (uint32_t)(m >> 1) & 1u)) ok = false;
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    aq_fence_after();
+                    if (!idle) aq_ld32(mine + b * 64, u[0]);
+                }
+                ahead = false;
                 if (!idle) {
-                    uint32_t u[64];
-                    aq_ld32(mine + b * 64, u);
-                    aq_ld32(mine + b * 64 + 32, u + 32);
-                    aq_ld_wait(u);
-                    aq_ld_wait(u + 32);
-                    const int key0 = (s.ta + i) * AS_KEYS;
-                    if (key0 + AS_KEYS > wmin) {                 // some row's keys end inside or before this tile
 #pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            if (key0 + e >= lim) u[e] = 0xff800000u;
-                    }
-                    float m4[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) m4[e] = __uint_as_float(u[e]);
-#pragma unroll
-                    for (int e = 4; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(u[e]));
-                    const float top = fmaxf(ref, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-                    if (__any_sync(0xffffffffu, (top - ref) * sl2 > 5.0f)) {
-                        const float corr = ref == -INFINITY ? 0.0f : ao_exp2((ref - top) * sl2);
-                        ref = top;
-                        sum *= corr;
-                        if (i > 0) {
-                            if (!mbar_wait_async(o_done + 2 * r + (b ^ 1), (uint32_t)((m - 1) >> 1) & 1u)) ok = false;
-                            ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) break;
-                            aq_fence_after();
-#pragma unroll 1
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t o[32];
-                                aq_ld32(mine + 128 + c * 32, o);
-                                aq_ld_wait(o);
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                aq_st32(mine + 128 + c * 32, o);
+                    for (int h = 0; h < 2; ++h) {
+                        aq_ld_wait(u[h]);
+                        if (h == 0) {
+                            aq_ld32(mine + b * 64 + 32, u[1]);
+                        } else if (i + 1 < cnt) {
+                            ahead = __all_sync(0xffffffffu, mbar_test(s_full + 2 * r + (b ^ 1), (uint32_t)((m + 1) >> 1) & 1u));
+                            if (ahead) {
+                                aq_fence_after();
+                                aq_ld32(mine + (b ^ 1) * 64, u[0]);
                             }
                         }
-                    }
-                    const float base = (ref == -INFINITY ? 0.0f : ref * sl2) - AO_LIFT;        // a row without any key so far
-                    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    uint32_t w[32];
+                        if (key0 + 32 * h + 32 > wmin) {         // some row's keys end inside or before these
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float a = ao_exp2(fmaf(__uint_as_float(u[2 * e]), sl2, -base)), c = ao_exp2(fmaf(__uint_as_float(u[2 * e + 1]), sl2, -base));
-                        s4[(2 * e) & 3] += a, s4[(2 * e + 1) & 3] += c;
-                        const __half2 h = __floats2half2_rn(a, c);
-                        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                            for (int e = 0; e < 32; ++e)
+                                if (key0 + 32 * h + e >= lim) u[h][e] = 0xff800000u;
+                        }
+                        float2 part[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+                        as_weights32(u[h], sl2, (ref == -INFINITY ? 0.0f : ref) - AO_LIFT, w[h], part);
+                        float all = (part[0].x + part[1].x) + (part[0].y + part[1].y);
+                        if (__any_sync(0xffffffffu, all > 32768.0f || (ref == -INFINITY && key0 + 32 * h < lim))) {
+                            const float now = fmaxf(ref, ceilf(as_top32(u[h]) * sl2)), corr = ref == -INFINITY ? 0.0f : ao_exp2(ref - now);
+                            ref = now;
+                            sum *= corr;
+                            if (h) {
+                                const __half2 c2 = __float2half2_rn(corr);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[0][e]), c2);
+                                    w[0][e] = *reinterpret_cast<const uint32_t*>(&x);
+                                }
+                                aq_st16(mine + b * 64, w[0]);
+                            }
+                            if (i > 0) {
+                                if (!mbar_wait_async(o_done + 2 * r + (b ^ 1), (uint32_t)((m - 1) >> 1) & 1u)) ok = false;
+                                ok = __all_sync(0xffffffffu, ok);
+                                if (!ok) break;
+                                aq_fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < 8; ++c) {
+                                    uint32_t lo[8], hi[8];
+                                    ts_ld16_issue(mine + 128 + c * 16, lo, hi);
+                                    ts_wait_ld(lo), ts_wait_ld(hi);
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e)
+                                        lo[e] = __float_as_uint(__uint_as_float(lo[e]) * corr), hi[e] = __float_as_uint(__uint_as_float(hi[e]) * corr);
+                                    ts_st8(mine + 128 + c * 16, lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]);
+                                    ts_st8(mine + 128 + c * 16 + 8, hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]);
+                                }
+                            }
+                            part[0] = part[1] = make_float2(0.0f, 0.0f);
+                            as_weights32(u[h], sl2, (ref == -INFINITY ? 0.0f : ref) - AO_LIFT, w[h], part);
+                            all = (part[0].x + part[1].x) + (part[0].y + part[1].y);
+                        }
+                        sum += all;
+                        aq_st16(mine + b * 64 + 16 * h, w[h]);   // (over scores that are in registers)
                     }
-                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-                    aq_st32(mine + b * 64, w);
+                    if (!ok) break;
                     aq_st_wait();
                 }
                 aq_fence_before();
@@ -427,8 +518,6 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
             const bool direct = s.place < 0;
             const float inv = 1.0f / sum;
             const bool on = sum > 0.0f || sum != sum;
-            int token = 0, head = 0;
-            const bool here = as_row(p, s, PROMPT, row, &token, &head);
             __half* dst = p.out + ((size_t)token * p.n_heads + head) * AO_D;
 #pragma unroll 1
             for (int c = 0; c < 4 && ok; ++c) {
@@ -458,22 +547,22 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                 }
                 __syncwarp();
             }
-            if (ok && !direct && here) as_store_ml(p, s.place, ROWS, row, ref == -INFINITY ? ref : ref * sl2 - AO_LIFT, sum);
+            if (ok && !direct && here) as_store_ml(p, s.place, ROWS, row, ref == -INFINITY ? ref : ref - AO_LIFT, sum);
+            mr += cnt;
+            if (!ok) break;
+            }
             aq_fence_before();
         }
-        __syncthreads();
-        aq_fence_after();
-        n0 += cnt;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-            if (i < sets) m0[i] += cnt;
-        if (*dead_s) {                                           // copies that were issued land before the CTA goes on
-            const long long c0 = clock64();
-            while (clock64() - c0 < (1LL << 22)) {}
-        }
-        if (*odd_s || *dead_s) as_multiply_out(p, s, PROMPT, ROWS, lim_s);
-        __syncthreads();
+    // ------------------------------ teardown ------------------------------
+    __syncthreads();
+    aq_fence_after();
+    if (*dead_s) {                                               // copies that were issued land before the CTA leaves
+        const long long c0 = clock64();
+        while (clock64() - c0 < (1LL << 22)) {}
     }
+    if (*dead_s || *odd_s)
+        for (int j = 0; as_piece<ROWS, PROMPT>(p, density, nsplit, j, s); ++j)
+            if (*dead_s || (*odd_s >> (j & 31)) & 1) as_multiply_out<PROMPT>(p, s, ROWS);
     if (warp == W::IWARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(W::COLS) : "memory");
 }
 

@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     const int from = f.g < 0 || place + f.n > p.places ? 0 : f.group.keys;     // tokens that the first kernel takes
     const int step = nsplit * AO_WARPS, chunks = (most + AO_KEYS - 1) / AO_KEYS;
     const uint32_t ring = smem_u32(ao_smem) + warp * (AO_STAGES * 2 * AO_HALF_STAGE);
+    const uint64_t policy = nrb == 1 ? ao_read_once() : ao_read_again();
     auto fetch = [&](int ch, int stage) {          // sixteen keys lie in one page
         if (ch < chunks) {
             const int key0 = ch * AO_KEYS, page = ao_page(p, slot, key0 >> p.c.page_shift);
@@ -155,8 +156,8 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
                 const int row = 2 * i + (lane >> 4);
                 const uint32_t d = dst + row * 256 + (((lane & 15) ^ (row & 7)) << 4);
                 const uint32_t n = page >= 0 && key0 + row < most ? 16u : 0u;      // (behind the last key: zeros)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(p.k + at + (size_t)row * AO_D), "r"(n) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + AO_HALF_STAGE), "l"(p.v + at + (size_t)row * AO_D), "r"(n) : "memory");
+                asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(d), "l"(p.k + at + (size_t)row * AO_D), "r"(n), "l"(policy) : "memory");
+                asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(d + AO_HALF_STAGE), "l"(p.v + at + (size_t)row * AO_D), "r"(n), "l"(policy) : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -346,7 +347,7 @@ static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int grou
     const long long rps = (long long)tps * (n_heads / c.n_kv);
     r.prompt = rps >= 64;
     if (r.prompt) {
-        r.rows = rps > 128 ? 256 : 128;
+        r.rows = 128;
         r.blocks = (int)(seqs * c.n_kv * ((rps + r.rows - 1) / r.rows));
         r.ctas = r.rows == 128 ? 2 * sm_count : sm_count;
         r.nsplit = std::max(1, std::min(64, r.ctas / r.blocks));

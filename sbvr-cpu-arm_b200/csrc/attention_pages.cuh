@@ -37,6 +37,18 @@ __device__ __forceinline__ float ao_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Keys and values that are read once leave L2 first: what every launch needs again (its instructions above all, tables, queries) stays.  With them in
+// the way, a launch on 4 x 8000 shared tokens stood for 9 us on instructions that came from DRAM behind the keys.
+__device__ __forceinline__ uint64_t ao_read_once() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ uint64_t ao_read_again() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
 __device__ __forceinline__ int ao_slot(const AoParams& p, int seq) {
     const int s = p.slots ? __ldg(p.slots + seq) : seq;
     return s >= 0 && s < p.c.max_seqs ? s : -1;

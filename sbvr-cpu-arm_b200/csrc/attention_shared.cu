@@ -99,6 +99,14 @@ __device__ __forceinline__ void as_weights32(const uint32_t* u, float sl2, float
     }
 }
 
+// One box of a 2-D tensor map, global -> shared, with a policy for L2
+__device__ __forceinline__ void as_tma_2d(void* dst_smem, const CUtensorMap* tmap, int c0, int c1, uint64_t* bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;"
+        ::"r"(smem_u32(dst_smem)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
+}
+
 struct AsSeg {                                     // a piece: what a CTA works on at a time
     int tok0, ntok;                                // tokens whose rows it has
     int row0, rows;                                // its first row among those of the first token, rows
@@ -107,6 +115,7 @@ struct AsSeg {                                     // a piece: what a CTA works 
     int keys;                                      // keys that any row attends to
     int least;                                     // ... that all rows do (which attend to any)
     int place;                                     // of its part, -1: the output
+    bool once;                                     // no other piece reads these keys
 };
 
 // row i of a piece -> token, query head
@@ -136,7 +145,7 @@ __device__ __forceinline__ bool as_piece(const AoParams& p, float density, int n
         s.tok0 += t0, s.row0 -= t0 * p.R;
         s.slot = ao_slot(p, seq);
         s.place = nsplit == 1 ? -1 : ((seq * p.c.n_kv + s.kvh) * nblk + blk) * nsplit + (int)blockIdx.x % nsplit;
-        s.keys = INT_MAX;
+        s.keys = INT_MAX, s.once = nblk == 1;
     } else {
         const int piece = (int)blockIdx.x + j * (int)gridDim.x;
         if (piece >= p.places) return false;                     // (only where groups overlap)
@@ -148,7 +157,7 @@ __device__ __forceinline__ bool as_piece(const AoParams& p, float density, int n
         const int seq = f.group.s0 + (seg - s.kvh * f.group.blocks) * p.per_block;
         s.tok0 = seq * p.tps, s.row0 = 0, s.rows = min(p.per_block, f.group.s1 - seq) * p.tps * p.R;
         s.slot = ao_slot(p, f.group.s0), s.keys = f.group.keys;
-        s.place = piece;
+        s.place = piece, s.once = f.group.blocks == 1;
     }
     s.ntok = (s.row0 + s.rows + p.R - 1) / p.R;
     int hi = 0, lo = INT_MAX;
@@ -292,6 +301,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
             int looked = 0;                                      // tiles of V that were looked through
             for (int j = 0; ok && as_piece<ROWS, PROMPT>(p, density, nsplit, j, s); ++j) {
               int y = entry(s.ta);
+              const uint64_t policy = s.once ? ao_read_once() : ao_read_again();
               for (int t = s.ta; t < s.tb; ++t, ++n0) {
                 const int b = n0 % ST, next = entry(t + 1);
                 if (n0 >= ST && (*dead_s || !mbar_wait_async(empty + b, (uint32_t)(n0 / ST - 1) & 1u))) ok = false;
@@ -305,8 +315,8 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                 if (lane == 0) mbar_arrive_expect_tx(bar, AS_TILE);
                 __syncwarp();
                 if (lane < boxes) {
-                    ts_tma_2d(dst + lane * box_bytes, is_k ? &kmap : &vmap, 0, y, bar);
-                    ts_tma_2d(dst + AS_KBOX + lane * box_bytes, is_k ? &kmap : &vmap, 64, y, bar);
+                    as_tma_2d(dst + lane * box_bytes, is_k ? &kmap : &vmap, 0, y, bar, policy);
+                    as_tma_2d(dst + AS_KBOX + lane * box_bytes, is_k ? &kmap : &vmap, 64, y, bar, policy);
                 }
                 __syncwarp();
                 if (look) {

@@ -120,8 +120,20 @@ __global__ void __launch_bounds__(128) pages_free_kernel(const PgCache c, const 
 }
 
 // ---------------------------------------------------------------------------------------------
-// reserve: one block.  scratch: [need prefix sums, n + 1][free pages]
+// reserve: one block.  scratch: [verdict][need prefix sums, n + 1][free pages].  More than PG_POSITIONS positions are written by a launch of their own behind
+// it (64 slots x 4000 by the one block: 60 us).
 // ---------------------------------------------------------------------------------------------
+constexpr int PG_POSITIONS = 8192;
+
+__global__ void __launch_bounds__(256) pages_positions_kernel(const PgCache c, const int* slots, const int* tokens, int each, int* positions, int tps) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int s = blockIdx.y, t = tokens ? tokens[s] : each;
+    const bool done = c.scratch[0] == 0;
+    const int first = done ? c.lengths[pg_slot(slots, s)] - t : 0, end = done ? t : 0;
+    for (int j = blockIdx.x * 256 + threadIdx.x; j < tps; j += gridDim.x * 256) positions[(size_t)s * tps + j] = j < end ? first + j : -1;
+}
+
 __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache c, const int* slots, const int* tokens, int each, int n,
                                                                    int* positions, int tps) {
     extern __shared__ uint32_t seen[];
@@ -129,8 +141,8 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache
     pdl_launch_dependents();
     pdl_wait();
     int fault = pg_slots_ok(c, slots, n, seen) ? 0 : SBVR_PAGES_BAD_SLOT;
-    int* first = c.scratch;                        // [n + 1]
-    int* list = c.scratch + c.max_seqs + 4;
+    int* first = c.scratch + 4;                    // [n + 1]
+    int* list = first + c.max_seqs + 4;
     int sum = 0;
     for (int base = 0; base < n; base += PG_THREADS) {
         const int i = base + threadIdx.x;
@@ -153,6 +165,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache
     if (!fault && sum > c.pages) fault = SBVR_PAGES_NO_PAGE;
     if (!fault && pg_find_free(c, sum, list, sc) < sum) fault = SBVR_PAGES_NO_PAGE;
     __syncthreads();
+    if (threadIdx.x == 0) c.scratch[0] = fault;
     if (fault) {
         if (threadIdx.x == 0) atomicOr(c.status, fault);
         if (positions)
@@ -181,46 +194,46 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache
 }
 
 // ---------------------------------------------------------------------------------------------
-// fork / copy: one block, then the copies.  scratch: [4: number of copies][first, n + 1][length of src, n][copies: src, dst, rows]
+// fork / copy: one block, then the copies.  scratch: [4: number of copies][free pages][copies: src, dst, rows]
 // ---------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(PG_THREADS) pages_fork_kernel(const PgCache c, const int* src, const int* dst, int n, int share) {
     extern __shared__ uint32_t seen[];
     __shared__ PgScan sc;
     pdl_launch_dependents();
     pdl_wait();
-    int* count = c.scratch;
-    int* first = c.scratch + 4;
-    int* slen = first + c.max_seqs + 4;
-    int* list = slen + c.max_seqs + 4;
+    // pairs in shared memory: slots, the parent's and the child's tokens, first page of the child's own
+    int* src_s = reinterpret_cast<int*>(seen + (c.max_seqs + 31) / 32);
+    int *dst_s = src_s + n, *slen = dst_s + n, *dlen = slen + n, *first = dlen + n;
+    int* list = c.scratch + 4;
     PgMove* moves = reinterpret_cast<PgMove*>(list + ((c.pages + 3) & ~3));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, me = threadIdx.x;
     bool ok = pg_slots_ok(c, dst, n, seen);
-    for (int i = threadIdx.x; i < n; i += PG_THREADS)
-        if (src[i] < 0 || src[i] >= c.max_seqs) ok = false;
-    int fault = __syncthreads_and(ok) ? 0 : SBVR_PAGES_BAD_SLOT;
-    int sum = 0;
-    for (int base = 0; base < n; base += PG_THREADS) {         // pages that every child needs of its own
-        const int i = base + threadIdx.x;
-        int need = 0;
-        if (i < n && !fault) {
-            const int len = max(c.lengths[src[i]], 0);
-            slen[i] = len;
-            if (src[i] != dst[i]) need = pg_pages_of(c, len) - (share ? min(len >> c.page_shift, c.max_pages) : 0);
+    int need = 0;
+    if (me < n) {                                  // (n <= 1024)
+        const int s = src[me], d = dst[me];
+        src_s[me] = s, dst_s[me] = d;
+        if (s < 0 || s >= c.max_seqs) {
+            ok = false;
+        } else if (ok) {
+            const int len = max(c.lengths[s], 0);
+            slen[me] = len, dlen[me] = c.lengths[d];
+            if (s != d) need = pg_pages_of(c, len) - (share ? min(len >> c.page_shift, c.max_pages) : 0);
         }
-        int total;
-        const int at = sum + pg_scan(sc, need, &total);
-        if (i < n) first[i] = at;
-        sum += total;
     }
-    if (threadIdx.x == 0) first[n] = sum;
+    int fault = __syncthreads_and(ok) ? 0 : SBVR_PAGES_BAD_SLOT, sum;
+    {
+        const int at = pg_scan(sc, fault ? 0 : need, &sum);
+        if (me < n) first[me] = at;
+        if (me == 0) first[n] = sum;
+    }
     if (!fault && sum > c.pages) fault = SBVR_PAGES_NO_PAGE;
     __syncthreads();
     auto counts = [&](int sign) {                  // what the children give up and what they take part in; pages that are read are held
         for (int i = warp; i < n; i += PG_THREADS / 32) {
-            if (src[i] == dst[i]) continue;
-            const int* rs = c.table + (size_t)src[i] * c.max_pages;
-            const int* rd = c.table + (size_t)dst[i] * c.max_pages;
-            const int have = pg_pages_of(c, c.lengths[dst[i]]), need = pg_pages_of(c, slen[i]);
+            if (src_s[i] == dst_s[i]) continue;
+            const int* rs = c.table + (size_t)src_s[i] * c.max_pages;
+            const int* rd = c.table + (size_t)dst_s[i] * c.max_pages;
+            const int have = pg_pages_of(c, dlen[i]), need = pg_pages_of(c, slen[i]);
             for (int k = lane; k < max(have, need); k += 32) {
                 const int o = k < have ? rd[k] : -1, s = k < need ? rs[k] : -1;
                 if (o == s) continue;
@@ -238,16 +251,16 @@ __global__ void __launch_bounds__(PG_THREADS) pages_fork_kernel(const PgCache c,
             fault = SBVR_PAGES_NO_PAGE;
         }
     }
-    if (threadIdx.x == 0) *count = fault ? 0 : sum;
+    if (threadIdx.x == 0) c.scratch[0] = fault ? 0 : sum;
     if (fault) {
         if (threadIdx.x == 0) atomicOr(c.status, fault);
         return;
     }
     for (int i = warp; i < n; i += PG_THREADS / 32) {          // pages of their own
-        if (src[i] == dst[i]) continue;
+        if (src_s[i] == dst_s[i]) continue;
         const int need = pg_pages_of(c, slen[i]), own = first[i + 1] - first[i], full = need - own;
         for (int j = lane; j < own; j += 32) {
-            const int s = c.table[(size_t)src[i] * c.max_pages + full + j], p = list[first[i] + j];
+            const int s = c.table[(size_t)src_s[i] * c.max_pages + full + j], p = list[first[i] + j];
             const bool on = s >= 0 && s < c.pages;
             c.refs[p] = 1;
             if (on) atomicSub(c.refs + s, 1);      // (no longer held)
@@ -260,7 +273,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_fork_kernel(const PgCache c,
     const int cols = PG_THREADS * PER / n;         // (n <= 1024)
     int most = 0;
     for (int i = threadIdx.x; i < n; i += PG_THREADS)
-        if (src[i] != dst[i]) most = max(most, max(pg_pages_of(c, slen[i]), pg_pages_of(c, c.lengths[dst[i]])));
+        if (src_s[i] != dst_s[i]) most = max(most, max(pg_pages_of(c, slen[i]), pg_pages_of(c, dlen[i])));
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) sc.warp[warp] = most;
     __syncthreads();
@@ -271,21 +284,21 @@ __global__ void __launch_bounds__(PG_THREADS) pages_fork_kernel(const PgCache c,
         for (int q = 0; q < PER; ++q) {
             const int e = q * PG_THREADS + threadIdx.x, i = e / cols, k = k0 + e % cols;
             v[q] = -2;
-            if (i >= n || k >= c.max_pages || src[i] == dst[i]) continue;
+            if (i >= n || k >= c.max_pages || src_s[i] == dst_s[i]) continue;
             const int need = pg_pages_of(c, slen[i]), full = need - (first[i + 1] - first[i]);
-            if (k < full) v[q] = c.table[(size_t)src[i] * c.max_pages + k];
+            if (k < full) v[q] = c.table[(size_t)src_s[i] * c.max_pages + k];
             else if (k < need) v[q] = list[first[i] + k - full];
-            else if (k < pg_pages_of(c, c.lengths[dst[i]])) v[q] = -1;
+            else if (k < pg_pages_of(c, dlen[i])) v[q] = -1;
         }
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const int e = q * PG_THREADS + threadIdx.x;
-            if (v[q] != -2) c.table[(size_t)dst[e / cols] * c.max_pages + k0 + e % cols] = v[q];
+            if (v[q] != -2) c.table[(size_t)dst_s[e / cols] * c.max_pages + k0 + e % cols] = v[q];
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < n; i += PG_THREADS) c.lengths[dst[i]] = slen[i];
+    if (me < n) c.lengths[dst_s[me]] = slen[me];
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -446,9 +459,18 @@ __global__ void __launch_bounds__(256) pages_rope_append_kernel(const PgCache c,
         x[0] = *reinterpret_cast<const uint4*>(p), x[1] = *reinterpret_cast<const uint4*>(p + PG_D / 2);
     };
     uint4 x[2][2];
+    int pos = -1;
+    if (tps > 1) {                                 // places without a token read nothing (half of a batch of uneven prompts)
+        pos = positions[t];
+        if (pos < 0) {
+            for (int it = threadIdx.x; it < n_heads * (PG_D / 8); it += 256)
+                *reinterpret_cast<uint4*>(q_out + (size_t)t * n_heads * PG_D + it * 8) = make_uint4(0u, 0u, 0u, 0u);
+            return;
+        }
+    }
     load(threadIdx.x, x[0]);
     load(threadIdx.x + 256, x[1]);
-    const int pos = positions[t];
+    if (tps == 1) pos = positions[t];
     if (threadIdx.x < PG_D / 2) {
         const double turn = (double)pos * (double)inv_freq[threadIdx.x];
         const float a = (float)fma(-rint(turn * 0.15915494309189535), 6.283185307179586, turn);
@@ -523,7 +545,7 @@ using namespace sbvr;
 
 static size_t seen_bytes(const PgCache& c) { return (size_t)(c.max_seqs + 31) / 32 * 4; }
 // where the copies stand in the scratch of a fork, and of a compaction
-static int fork_moves_at(const PgCache& c) { return 4 + 2 * (c.max_seqs + 4) + ((c.pages + 3) & ~3); }
+static int fork_moves_at(const PgCache& c) { return 4 + ((c.pages + 3) & ~3); }
 static int compact_moves_at(const PgCache& c) { return 4 + 2 * ((c.pages + 3) & ~3); }
 
 static int launch_moves(const PgCache& c, int list_at, int place_at, cudaStream_t st) {
@@ -561,8 +583,13 @@ int sbvr_pages_reserve(const sbvr_pages_t* cache, const int* slots, const int* t
     if (rc) return rc;
     if (n < 1 || n > c.max_seqs || (!tokens && tokens_each < 0) || (positions && tokens_per_seq < 1)) return SBVR_ERR_BAD_ARG;
     if (positions && (long long)n * tokens_per_seq > INT_MAX / 2) return SBVR_ERR_UNSUPPORTED;
+    const bool many = positions && (long long)n * tokens_per_seq > PG_POSITIONS;
+    if (many && n > 65535) return SBVR_ERR_UNSUPPORTED;
     SBVR_CUDA_TRY(launch_pdl(pages_reserve_kernel, dim3(1), dim3(PG_THREADS), seen_bytes(c), reinterpret_cast<cudaStream_t>(stream), c, slots, tokens,
-                             tokens_each, n, positions, tokens_per_seq));
+                             tokens_each, n, many ? nullptr : positions, tokens_per_seq));
+    if (many)
+        SBVR_CUDA_TRY(launch_pdl(pages_positions_kernel, dim3((unsigned)std::min((tokens_per_seq + 1023) / 1024, 64), (unsigned)n), dim3(256), 0,
+                                 reinterpret_cast<cudaStream_t>(stream), c, slots, tokens, tokens_each, positions, tokens_per_seq));
     return SBVR_OK;
 }
 
@@ -572,7 +599,7 @@ int sbvr_pages_fork(const sbvr_pages_t* cache, const int* src, const int* dst, i
     if (rc) return rc;
     if (!src || !dst || n < 1 || n > c.max_seqs) return SBVR_ERR_BAD_ARG;
     if (n > PG_THREADS) return SBVR_ERR_UNSUPPORTED;
-    SBVR_CUDA_TRY(launch_pdl(pages_fork_kernel, dim3(1), dim3(PG_THREADS), seen_bytes(c), reinterpret_cast<cudaStream_t>(stream), c, src, dst, n, share ? 1 : 0));
+    SBVR_CUDA_TRY(launch_pdl(pages_fork_kernel, dim3(1), dim3(PG_THREADS), seen_bytes(c) + (5 * (size_t)n + 1) * 4, reinterpret_cast<cudaStream_t>(stream), c, src, dst, n, share ? 1 : 0));
     return launch_moves(c, fork_moves_at(c), 0, reinterpret_cast<cudaStream_t>(stream));
 }
 

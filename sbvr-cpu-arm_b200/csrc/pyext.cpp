@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -416,7 +417,7 @@ const int* ints(const at::Tensor& t) { return t.defined() ? t.data_ptr<int>() : 
 // pages_reserve(cache, device, slots, n, tokens (tensor or int), tokens_per_seq) -> positions or None
 PyObject* py_pages_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        c10::InferenceMode im;
+        c10::AutoGradMode grad(false);
         Pages p(a, n, 6, "pages_reserve");
         int64_t k = as_int(a[3]);
         at::Tensor slots = p.slots(a[2], &k), tokens, positions;
@@ -464,7 +465,7 @@ PyObject* py_pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // pages_common(cache, device, slots, n, group_starts) -> shared
 PyObject* py_pages_common(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        c10::InferenceMode im;
+        c10::AutoGradMode grad(false);
         Pages p(a, n, 5, "pages_common");
         int64_t k = as_int(a[3]);
         at::Tensor slots = p.slots(a[2], &k), starts = p.need(a[4], at::kInt, "group_starts");
@@ -485,7 +486,7 @@ int64_t seqs_of(const Pages& p, const at::Tensor& slots, const at::Tensor& posit
 // pages_rope_append(cache, device, layer, qkv, positions, inv_freq, scaling, slots, n, q_out) -> q
 PyObject* py_pages_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        c10::InferenceMode im;
+        c10::AutoGradMode grad(false);
         Pages p(a, n, 10, "pages_rope_append");
         at::Tensor qkv = p.need(a[3], at::kHalf, "qkv"), pos = p.need(a[4], at::kInt, "positions"), inv = p.need(a[5], at::kFloat, "inv_freq");
         const double scaling = PyFloat_AsDouble(a[6]);
@@ -506,7 +507,7 @@ PyObject* py_pages_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // pages_attention(cache, device, layer, q, positions, slots, n, scale, group_starts, shared, out) -> out
 PyObject* py_pages_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        c10::InferenceMode im;
+        c10::AutoGradMode grad(false);
         Pages p(a, n, 11, "pages_attention");
         at::Tensor q = opt_tensor(a[3], "q"), pos = p.need(a[4], at::kInt, "positions"), slots = p.tensor(a[5], at::kInt, "slots");
         const double scale = PyFloat_AsDouble(a[7]);

@@ -29,6 +29,7 @@ from sbvr.core import linear as sbvr_linear
 from sbvr.core import sbvr as sbvr_tensor
 
 from . import parallel
+from .pages import PagedCache
 
 
 @dataclass
@@ -205,6 +206,8 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
         self._bufs = {}
         self._graph = None
         self._stream = None
+        self.pages: Optional[PagedCache] = None    # of generate_shared (attach_pages)
+        self._shared_graph = None
         self._comm = None
         self.fuse_glue = True                      # fold norm / SiLU into the decode linears where the kernel allows
         self.pushed_allreduce = True               # tensor-parallel decode: results pushed to the peers by the GEMV itself
@@ -372,7 +375,11 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             else:
                 norm_linear(layer.qkv_proj, delta, layer.input_layernorm_weight, b.qkv)
             att_scratch = None if b.att_scratch is None else b.att_scratch.data_ptr()
-            if tokens_per_seq == 1 and self.fuse_glue:     # decode: rotary embedding and cache append inside attention
+            paged = b.extra.get("paged")
+            if paged is not None:                          # the cache in pages: what the sequences share is read once for all of them
+                q = self.pages.rope_append(li, b.qkv, b.positions, self.inv_freq, paged["slots"], float(self.attention_scaling), q_out=paged["q"])
+                self.pages.attention(li, q, b.positions, paged["slots"], scale, paged["starts"], paged["shared"], out=b.ao)
+            elif tokens_per_seq == 1 and self.fuse_glue:     # decode: rotary embedding and cache append inside attention
                 ck(L.sbvr_rope_attention_f16(b.qkv.data_ptr(), b.positions.data_ptr(), self.inv_freq.data_ptr(),
                                              float(self.attention_scaling), self.kcache[li].data_ptr(),
                                              self.vcache[li].data_ptr(), b.ao.data_ptr(), att_scratch, T, self.n_heads,
@@ -428,7 +435,10 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             if not normed:
                 ck(L.sbvr_add_rmsnorm_f16(hc.data_ptr(), None if delta is None else delta.data_ptr(),
                                           self.norm_weight.data_ptr(), None, b.xn.data_ptr(), T, H, eps, st), "rmsnorm")
-            rows = b.xn.view(-1, tokens_per_seq, H)[:, -1, :].contiguous() if rows_sel else b.xn
+            rows = b.xn
+            if rows_sel:
+                last = b.extra.get("last")                 # uneven prompts: their last tokens
+                rows = b.xn.view(-1, tokens_per_seq, H)[:, -1, :].contiguous() if last is None else b.xn.index_select(0, last)
             self.lm_head(rows, out=b.logits)
         else:
             norm_linear(self.lm_head, delta, self.norm_weight, b.logits, keep_residual=False)
@@ -525,6 +535,104 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             out[:, i] = b.next_ids
         self._check()
         return out
+
+    # ------------------------------------------------------------------ sequences that begin alike
+    def attach_pages(self, pages: int, page_size: int = 64, max_seqs: Optional[int] = None, max_pages: Optional[int] = None) -> PagedCache:
+        """Gives the model a cache in pages for `generate_shared` (beside the dense one of `generate`, which may be built for few tokens)."""
+        self._shared_graph = None
+        for key in [k for k in self._bufs if k[0] == "paged"]:
+            del self._bufs[key]
+        self.pages = PagedCache(self.config.num_hidden_layers, self.n_kv, pages, page_size, max_seqs or self.max_batch, max_pages,
+                                self.config.head_dim, self.device)
+        return self.pages
+
+    def _act_paged(self, tokens: int, rows_out: int, seqs: int) -> _Buffers:
+        key = ("paged", tokens, rows_out, seqs)
+        b = self._bufs.get(key)
+        if b is None:
+            plain = self._bufs.pop((tokens, rows_out), None)
+            b = self._act(tokens, rows_out)
+            del self._bufs[(tokens, rows_out)]
+            if plain is not None:
+                self._bufs[(tokens, rows_out)] = plain
+            i32 = dict(dtype=torch.int32, device=self.device)
+            b.extra["paged"] = {"slots": torch.arange(seqs, **i32), "starts": torch.tensor([0, seqs], **i32), "shared": torch.zeros(1, **i32),
+                                "q": torch.empty((tokens, self.n_heads * self.config.head_dim), dtype=torch.float16, device=self.device)}
+            self._bufs[key] = b
+        return b
+
+    def _shared_step(self, b: _Buffers):
+        """One decode step of all sequences: room for a token each, the step, its tokens as the next one's."""
+        b.positions.copy_(self.pages.reserve(b.extra["paged"]["slots"], 1, tokens_per_seq=1))
+        self._forward_rows(b, 1, last_only=True)
+        b.ids.copy_(b.next_ids)
+
+    @torch.inference_mode()
+    def generate_shared(self, prefix_ids: torch.Tensor, prompt_ids: torch.Tensor, max_new_tokens: int,
+                        prompt_lengths: Optional[torch.Tensor] = None, use_graph: bool = True) -> torch.Tensor:
+        """Greedy generation for prompts that begin alike: `prefix_ids` [L] is run once and held once, every row of `prompt_ids` [B, P] (its first
+        `prompt_lengths[i]` >= 1 tokens; all of them by default) goes on from it.  Needs `attach_pages`; uses its slots 0 .. B - 1, which hold nothing
+        before and after.  Returns [B, max_new_tokens] int32."""
+        cache = self.pages
+        if cache is None:
+            raise RuntimeError("generate_shared needs a cache in pages: call attach_pages first")
+        B, P = prompt_ids.shape
+        L, page = prefix_ids.numel(), cache.page_size
+        lens = [P] * B if prompt_lengths is None else [int(n) for n in prompt_lengths]
+        if B < 1 or P < 1 or max_new_tokens < 1 or len(lens) != B or min(lens) < 1 or max(lens) > P:
+            raise ValueError("every prompt needs at least one token, and no more than its row holds")
+        whole = L // page
+        need = [-(-(L + n + max_new_tokens - 1) // page) for n in lens]
+        if B > cache.max_seqs or max(need) > cache.max_pages or whole + sum(n - whole for n in need) > cache.pages:
+            raise ValueError("sequences beyond the cache in pages that this model was given")
+        out = torch.empty((B, max_new_tokens), dtype=torch.int32, device=self.device)
+        if L:                                      # the common beginning, once, in slot 0
+            b = self._act_paged(L, 1, 1)
+            b.ids.copy_(prefix_ids.reshape(-1).to(torch.int32))
+            b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], L, tokens_per_seq=L))
+            b.extra["paged"]["shared"].zero_()
+            self._forward_rows(b, L, last_only=True)
+            if B > 1:
+                cache.fork([0] * (B - 1), list(range(1, B)))
+        d = self._act_paged(B, B, B)
+        d.extra["paged"]["shared"].copy_(cache.common(d.extra["paged"]["slots"], d.extra["paged"]["starts"]))
+        b = self._act_paged(B * P, B, B) if P > 1 else d
+        b.ids.copy_(prompt_ids.reshape(-1).to(torch.int32))
+        b.extra["paged"]["shared"].copy_(d.extra["paged"]["shared"])
+        b.extra["last"] = torch.tensor([i * P + n - 1 for i, n in enumerate(lens)], device=self.device) if P > 1 else None
+        b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], torch.tensor(lens, dtype=torch.int32, device=self.device), tokens_per_seq=P))
+        self._forward_rows(b, P, last_only=True)
+        out[:, 0] = b.next_ids
+        d.ids.copy_(b.next_ids)
+        if max_new_tokens > 1:
+            if use_graph and (self._shared_graph is None or self._shared_graph[0] != B):
+                self._shared_graph = (B, self._capture_shared(d))
+            for i in range(1, max_new_tokens):
+                if use_graph:
+                    self._shared_graph[1].replay()
+                else:
+                    self._shared_step(d)
+                out[:, i] = d.ids
+        cache.free(d.extra["paged"]["slots"])
+        self._check()
+        cache.check()
+        return out
+
+    def _capture_shared(self, d: _Buffers):
+        """Captures one decode step on the cache in pages; the warm-up step's tokens are given back (their pages are written again)."""
+        s = torch.cuda.Stream(device=self.device)
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            book, ids = self.pages.book.clone(), d.ids.clone()
+            self._shared_step(d)
+            self.pages.book.copy_(book)
+            d.ids.copy_(ids)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s, capture_error_mode="thread_local"):
+                self._shared_step(d)
+        torch.cuda.current_stream().wait_stream(s)
+        return g
 
     def _check(self):
         torch.cuda.synchronize(self.device)

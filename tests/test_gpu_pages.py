@@ -271,3 +271,218 @@ def test_attention(case):
     empty = pos < 0
     assert not out[1:-1][empty].any()
     c.check()
+
+
+@pytest.mark.parametrize("case", [(1, 3, 90, 70, 64, 8, 4, 32), (1, 5, 300, 40, 40, 8, 2, 16), (1, 4, 200, 30, 6, 8, 2, 16), (2, 9, 640, 20, 1, 8, 2, 128)])
+def test_what_lies_behind_a_sequence_does_not_matter(case):
+    """Finite leftovers, infinities and NaN behind the last token and in free pages: the same bits."""
+    outs = []
+    for fill in (0.0, 60000.0, float("inf"), float("nan")):
+        c, q, pos, slots, starts = batch(*case, seed=77)
+        c.pool[torch.isnan(c.pool)] = fill
+        outs.append(c.attention(0, q, pos, slots, group_starts=starts, shared=c.common(slots, starts)))
+    assert torch.isfinite(outs[0]).all() and all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("tps,groups", [(6, True), (6, False), (60, False), (1, True), (5, True)])
+def test_values_that_are_not_finite_reach_the_tokens_that_see_them(tps, groups):
+    c, q, pos, slots, starts = batch(1, 4, 256, 60, tps, 8, 2, 32, seed=5)
+    common = c.common(slots, starts)
+    say = dict(group_starts=starts, shared=common) if groups else {}
+    o, mag = attention(c, 0, q, pos, slots, 8)                 # (dims do not mix: those that stay finite stay what they are)
+    at = int(pos.view(4, tps)[0, tps // 2])                    # the first sequence's own, seen from the middle token on
+    page = int(c.table[slots[0], at // 32])
+    c.pool[0, 1, page, 1, at % 32, 3] = float("inf")
+    c.pool[0, 1, int(c.table[slots[0], 2]), 0, 5, 7] = float("-inf")           # a shared one, seen by all
+    got = c.attention(0, q, pos, slots, **say).view(4, tps, 2, 4, D)
+    bad = ~torch.isfinite(got)
+    expect = torch.zeros_like(bad)
+    expect[0, tps // 2:, 1, :, 3] = True
+    expect[..., 0, :, 7] = True
+    expect[pos.view(4, tps) < 0] = False
+    assert torch.equal(bad, expect)
+    bad = bad.view(4 * tps, -1)
+    close(got.view(4 * tps, -1).masked_fill(bad, 0), (o.masked_fill(bad, 0), mag), 316)
+
+
+@pytest.mark.parametrize("step", [0.02, 0.7, 9.0])
+@pytest.mark.parametrize("tps", [1, 40])
+def test_growing_scores(step, tps):
+    """Scores that grow along the keys, slowly and fast: the reference of the weights lags behind and is moved in steps."""
+    c, q, pos, slots, starts = batch(1, 5, 640, 90, tps, 8, 2, 64, seed=9)
+    n = 730
+    q *= 0.1
+    q.view(-1, 8, D)[:, :, 0] = 8.0
+    ramp = (torch.arange(n, device="cuda") * step * D ** 0.5 / 8.0).clamp(max=30000.0).half()
+    for s in slots:
+        for k in range(-(-n // 64)):
+            p = int(c.table[s, k])
+            if p >= 0:
+                c.pool[0, 0, p, :, :, 0] = ramp[k * 64:(k + 1) * 64].new_zeros(64).copy_(torch.nn.functional.pad(ramp[k * 64:(k + 1) * 64], (0, max(0, (k + 1) * 64 - n))))
+    common = c.common(slots, starts)
+    o, mag = attention(c, 0, q, pos, slots, 8)
+    out = c.attention(0, q, pos, slots, group_starts=starts, shared=common)
+    # fp32 scores of up to 9 * 730 * log2(e): half a step of 2^-11 of them at most, in the exponent; eight products' and sums' worth
+    slack = 1.0 + 8 * 2.0 ** -24 * (n * step * 1.4427) * 2.0 ** 11
+    err = (out.double() - o).abs()
+    assert (err <= slack * HALF * (mag + o.abs()) + 2.0 ** -24).all(), (err / (mag + o.abs() + 1e-9)).max()
+
+
+def test_rows_apart_and_scales():
+    c, q, pos, slots, starts = batch(1, 6, 300, 40, 2, 8, 2, 32, seed=11)
+    common = c.common(slots, starts)
+    wide = torch.full((q.shape[0], q.shape[1] + 3 * 8), 9.0, dtype=torch.float16, device="cuda")
+    wide[:, 8:8 + q.shape[1]] = q
+    view = wide[:, 8:8 + q.shape[1]]
+    assert torch.equal(c.attention(0, q, pos, slots, group_starts=starts, shared=common), c.attention(0, view, pos, slots, group_starts=starts, shared=common))
+    for scale in (0.01, 1.0):
+        close(c.attention(0, q, pos, slots, scale=scale, group_starts=starts, shared=common), attention(c, 0, q, pos, slots, 8, scale), 340 if scale < 1 else 3400)
+
+
+def test_any_batch_order_and_groups():
+    """Groups of one, groups that share nothing, sequences in no group, a slot twice in a batch."""
+    c, q, pos, slots, starts = batch(3, 4, 200, 50, 1, 8, 2, 16, seed=13)
+    ref = attention(c, 0, q, pos, slots, 8)
+    for cuts in ([0, 4, 8, 12], [0, 1, 4, 12], [2, 4], [0, 2, 8], [5, 5, 8, 8, 12]):
+        g = ints(cuts)
+        close(c.attention(0, q, pos, slots, group_starts=g, shared=c.common(slots, g)), ref, 250)
+    twice = [slots[0], slots[0], slots[5], slots[0]]
+    rows = [0, 0, 5, 0]
+    out = c.attention(0, q[rows].contiguous(), pos[rows].contiguous(), ints(twice), group_starts=ints([0, 2, 4]), shared=c.common(ints(twice), ints([0, 2, 4])))
+    close(out, (ref[0][rows], ref[1][rows]), 250)
+    assert torch.equal(out[0], out[1])
+
+
+def test_many_groups():
+    c, q, pos, slots, starts = batch(70, 2, 40, 6, 1, 4, 2, 16, seed=15)
+    close(c.attention(0, q, pos, slots, group_starts=starts, shared=c.common(slots, starts)), attention(c, 0, q, pos, slots, 4), 46)
+
+
+def test_a_far_layer():
+    """Elements of a pool beyond 2^31."""
+    c, q, pos, slots, starts = batch(1, 3, 500, 60, 1, 8, 8, 256, seed=17, layers=2, spare=5000)
+    assert c.pool[1].storage_offset() + c.pool[1].numel() > 2 ** 31
+    c.pool[1, :, c.refs > 0] = c.pool[0, :, c.refs > 0]
+    a, b = (c.attention(layer, q, pos, slots, group_starts=starts, shared=c.common(slots, starts)) for layer in (0, 1))
+    assert torch.equal(a, b)
+    close(b, attention(c, 1, q, pos, slots, 8), 560)
+
+
+def test_replayed_and_on_other_streams():
+    """Two graphs of the same cache replayed one after the other, and a call on a stream of its own: the same bits as the eager call."""
+    c, q, pos, slots, starts = batch(2, 20, 700, 90, 1, 32, 8, 64, seed=19)
+    sl, common = ints(slots), c.common(slots, starts)
+    want = c.attention(0, q, pos, sl, group_starts=starts, shared=common)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = c.attention(0, q, pos, sl, group_starts=starts, shared=common)
+        graphs.append((g, out))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = c.attention(0, q, pos, sl, group_starts=starts, shared=common)
+    for _ in range(3):
+        for g, out in graphs:
+            out.zero_()
+            g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(other, want) and all(torch.equal(out, want) for _, out in graphs)
+
+
+def test_two_calls_at_once():
+    """Two streams, two batches, one cache that neither changes: every call has scratch of its own."""
+    c, q, pos, slots, starts = batch(2, 20, 3000, 90, 1, 32, 8, 64, seed=21)
+    sl, common = ints(slots), c.common(slots, starts)
+    q2 = q.flip(0).contiguous()
+    want = [c.attention(0, x, pos, sl, group_starts=starts, shared=common) for x in (q, q2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(c.attention(0, (q, q2)[k], pos, sl, group_starts=starts, shared=common))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[k]) for k in range(2) for o in got[k])
+
+
+def test_refusals():
+    from sbvr import _lib
+    c, q, pos, slots, starts = batch(1, 4, 64, 20, 1, 8, 2, 16, seed=23)
+    common = c.common(slots, starts)
+    inv = torch.ones(64, device="cuda")
+    qkv = torch.zeros((4, 12 * D), dtype=torch.float16, device="cuda")
+    before = c.pool.clone()
+    for call in (lambda: c.attention(1, q, pos, slots), lambda: c.attention(-1, q, pos, slots), lambda: c.attention(0, q[:, :-D], pos, slots),
+                 lambda: c.attention(0, q, pos, slots, scale=0.0), lambda: c.attention(0, q, pos, slots, scale=float("nan")),
+                 lambda: c.attention(0, q, pos, slots, scale=-0.1), lambda: c.rope_append(1, qkv, pos, inv, slots)):
+        with pytest.raises(RuntimeError):
+            call()
+    for call in (lambda: c.attention(0, q.float(), pos, slots), lambda: c.attention(0, q.cpu(), pos, slots), lambda: c.attention(0, q[:3], pos, slots),
+                 lambda: c.attention(0, q, pos.long(), slots), lambda: c.attention(0, q, pos, slots, group_starts=starts),
+                 lambda: c.attention(0, q, pos, slots, group_starts=starts[:1], shared=common), lambda: c.attention(0, q.t(), pos, slots),
+                 lambda: c.attention(0, q, pos[:3], slots), lambda: c.attention(0, q, pos, slots, out=q[:2]), lambda: c.rope_append(0, qkv[:, :-8], pos, inv, slots),
+                 lambda: c.rope_append(0, qkv, pos, inv[:-1], slots), lambda: c.reserve([0, 1], ints([1])), lambda: c.fork([0], [1, 2]),
+                 lambda: c.common(slots, starts[:1]), lambda: c.free([9]), lambda: c.fork([0, 1], [2, 2]), lambda: c.reserve([0], -1), lambda: c.free([])):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+    lib, st = _lib.lib, torch.cuda.current_stream().cuda_stream
+    out = torch.zeros_like(q)
+    args = [c._at, 0, q.data_ptr(), 8 * D, None, pos.data_ptr(), None, None, 0, out.data_ptr(), None, 0, 4, 1, 8, 0.1, st]
+    import ctypes
+
+    def with_(i, v):
+        a = list(args)
+        a[i] = v
+        return lib.sbvr_pages_attention_f16(ctypes.cast(a[0], ctypes.POINTER(_lib.Pages)), *a[1:])
+    assert with_(12, 4) == 0 and with_(12, 0) == -1 and with_(14, 7) == -1 and with_(12, 6) == -1 and with_(3, 8 * D - 8) == -1
+    assert with_(3, 8 * D + 1) == -3 and with_(2, q.data_ptr() + 2) == -3 and with_(5, None) == -1 and with_(8, 2) == -1
+    torch.cuda.synchronize()
+    assert torch.equal(c.pool.view(torch.int16), before.view(torch.int16))
+    with pytest.raises(RuntimeError, match="no page"):           # (of the one call that was taken: it reads slot i for sequence i, and one of them is empty)
+        c.check()
+
+
+# ------------------------------------------------------------------ together
+def tiny(seed=3, **kw):
+    from models.sbvr_llama import LlamaConfig, SBVRLlamaForCausalLM
+    return SBVRLlamaForCausalLM(LlamaConfig.preset("tiny"), device="cuda", max_batch=8, max_ctx=400, **kw).init_synthetic(seed)
+
+
+@pytest.mark.parametrize("L,B,P,page", [(100, 5, 9, 16), (33, 1, 1, 32), (0, 3, 7, 16), (200, 8, 40, 64)])
+def test_generate_shared(L, B, P, page):
+    """A prefix once and prompts of uneven lengths: a captured step equals an eager one, and the logits are those of the dense cache (two fp16 layers,
+    whose rotary embeddings round differently: 1e-2, the bound of this model's outputs)."""
+    m = tiny()
+    c = m.attach_pages(60, page, max_seqs=8)
+    g = torch.Generator(device="cuda").manual_seed(L)
+    prefix = torch.randint(0, 1024, (L,), device="cuda", generator=g)
+    prompts = torch.randint(0, 1024, (B, P), device="cuda", generator=g)
+    lens = [P] + [1 + (7 * i) % P for i in range(1, B)]
+    got = m.generate_shared(prefix, prompts, 6, prompt_lengths=lens)
+    assert got.shape == (B, 6)
+    assert torch.equal(got, m.generate_shared(prefix, prompts, 6, prompt_lengths=lens, use_graph=False))
+    assert torch.equal(got, m.generate_shared(prefix, prompts, 6, prompt_lengths=torch.tensor(lens)))
+    assert not c.refs.any() and not c.lengths.any() and (c.table == -1).all()
+    m.generate_shared(prefix, prompts, 1, prompt_lengths=lens)
+    logits = m._bufs[("paged", B * P, B, B)].logits.double()
+    for i in range(B):
+        ids = torch.cat((prefix, prompts[i, :lens[i]]))[None]
+        want = m.forward(ids)[0, -1].double()
+        assert (logits[i] - want).norm() / want.norm() < 1e-2
+
+
+def test_generate_shared_refuses_what_does_not_fit():
+    m = tiny()
+    ids = torch.zeros((2, 5), dtype=torch.long, device="cuda")
+    with pytest.raises(RuntimeError, match="attach_pages"):
+        m.generate_shared(ids[0], ids, 2)
+    m.attach_pages(6, 16, max_seqs=2)
+    for args in ((ids[0], ids[:, :0], 2), (ids[0], ids, 0), (ids[0], ids.repeat(2, 1), 2), (ids[0], ids, 92)):
+        with pytest.raises(ValueError):
+            m.generate_shared(*args)
+    with pytest.raises(ValueError):
+        m.generate_shared(ids[0], ids, 2, prompt_lengths=[5, 0])
+    assert m.generate_shared(ids[0], ids, 2).shape == (2, 2)

@@ -364,8 +364,8 @@ static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int grou
             r.places = (size_t)r.blocks + AS_ROUNDS * r.ctas;  // (ao_density)
         }
         const long long units = (long long)seqs * c.n_kv * ((rps + 15) / 16);
-        r.nsplit = 1;                              // CTAs on a sequence's own keys: as many as make about two per SM, at most 8
-        while (r.nsplit < 8 && units * r.nsplit * 2 <= 2 * sm_count) r.nsplit *= 2;
+        r.nsplit = 1;                              // CTAs on a sequence's own keys: as many as make about two per SM, at most 16 (a cluster)
+        while (r.nsplit < 16 && units * r.nsplit * 2 <= 2 * sm_count) r.nsplit *= 2;
     }
     return r;
 }
@@ -423,8 +423,9 @@ int sbvr_pages_attention_f16(const sbvr_pages_t* cache, int layer, const void* q
         if (r.nsplit > 1) SBVR_CUDA_TRY(launch_pdl(attention_join_kernel, dim3((unsigned)(r.blocks * (r.rows / 32))), dim3(256), 0, st, p, r.nsplit));
         return SBVR_OK;
     }
-    static SmemOnce once;
+    static SmemOnce once, once_cluster;
     rc = set_max_smem_once(once, attention_own_kernel, AO_SMEM);
+    if (!rc) rc = set_attribute_once(once_cluster, attention_own_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);      // (clusters of 16)
     if (rc) return rc;
     const int units = seqs * c.n_kv * ((p.tps * p.R + 15) / 16);
     SBVR_CUDA_TRY(launch_pdl_cluster(attention_own_kernel, dim3((unsigned)(units * r.nsplit)), dim3(AO_WARPS * 32), r.nsplit, (size_t)AO_SMEM, st, p, r.nsplit));

@@ -439,12 +439,12 @@ SBVR_API int sbvr_pages_compact(const sbvr_pages_t* cache, sbvr_stream_t stream)
 SBVR_API int sbvr_pages_common(const sbvr_pages_t* cache, const int* slots, int n, const int* group_starts, int groups, int* shared,
                                sbvr_stream_t stream);
 /* As sbvr_rope_append_f16, to pages: q_out[token][n_heads * 128] = the rotated queries (zeros for a position below 0), k and v go to the pages of
- * slots[token / tokens_per_seq] at positions[token] (below 0: nowhere).  qkv is left as it is.  Angles in 64 bits, the rotation in 32, one rounding. */
+ * slots[token / tokens_per_seq] at positions[token] (below 0: nowhere).  qkv is left as it is; q_out must not overlap it.  Angles in 64 bits, the rotation in 32, one rounding. */
 SBVR_API int sbvr_pages_rope_append_f16(const sbvr_pages_t* cache, int layer, const void* qkv, const int* positions, const float* inv_freq,
                                         float attn_scaling, const int* slots, int seqs, int tokens_per_seq, int n_heads, void* q_out,
                                         sbvr_stream_t stream);
 /* out[token][head] = softmax(q . K^T * scale) . V over positions 0 .. positions[token] of the slot of sequence token / tokens_per_seq (none below 0:
- * zeros).  q rows q_pitch elements apart (a multiple of 8), out [seqs * tokens_per_seq][n_heads * 128]; n_heads a multiple of n_kv; scale > 0.
+ * zeros).  q rows q_pitch elements apart (a multiple of 8), out [seqs * tokens_per_seq][n_heads * 128], which must not overlap q; n_heads a multiple of n_kv; scale > 0.
  * groups > 0: sequences group_starts[g] .. group_starts[g + 1] - 1 hold their first shared[g] tokens (whole pages count) in the same pages, those of
  * the group's first sequence are read, once for all of them (sbvr_pages_common finds them); sequences in no group share nothing.  groups = 0: nothing is shared.
  * scratch: sbvr_pages_attention_scratch_bytes(), 16-byte aligned, not used by another call at the same time. */

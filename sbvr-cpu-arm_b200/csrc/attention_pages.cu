@@ -401,6 +401,8 @@ int sbvr_pages_attention_f16(const sbvr_pages_t* cache, int layer, const void* q
     if (!slots && seqs > c.max_seqs) return SBVR_ERR_BAD_ARG;
     if ((long long)seqs * tokens_per_seq > INT_MAX / 4 / n_heads) return SBVR_ERR_UNSUPPORTED;
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) & 15) || q_pitch % 8) return SBVR_ERR_ALIGN;
+    const size_t tokens = (size_t)seqs * tokens_per_seq;         // other CTAs still read q while out is written
+    if (pg_overlap(q, ((tokens - 1) * q_pitch + (size_t)n_heads * AO_D) * 2, out, tokens * n_heads * AO_D * 2)) return SBVR_ERR_BAD_ARG;
     DeviceInfo di;
     int dev = 0;
     SBVR_CUDA_TRY(cudaGetDevice(&dev));

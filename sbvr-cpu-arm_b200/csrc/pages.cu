@@ -630,6 +630,8 @@ int sbvr_pages_rope_append_f16(const sbvr_pages_t* cache, int layer, const void*
     if (!slots && seqs > c.max_seqs) return SBVR_ERR_BAD_ARG;
     if ((long long)seqs * tokens_per_seq > INT_MAX / 2 || (long long)n_heads + 2 * c.n_kv > INT_MAX / 16) return SBVR_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) return SBVR_ERR_ALIGN;
+    const size_t tokens = (size_t)seqs * tokens_per_seq;
+    if (pg_overlap(qkv, tokens * (n_heads + 2 * c.n_kv) * PG_D * 2, q_out, tokens * n_heads * PG_D * 2)) return SBVR_ERR_BAD_ARG;
     SBVR_CUDA_TRY(launch_pdl(pages_rope_append_kernel, dim3((unsigned)(seqs * tokens_per_seq)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), c, layer,
                              static_cast<const __half*>(qkv), positions, inv_freq, attn_scaling, slots, tokens_per_seq, n_heads, static_cast<__half*>(q_out)));
     return SBVR_OK;

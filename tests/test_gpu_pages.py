@@ -408,6 +408,56 @@ def test_two_calls_at_once():
     assert all(torch.equal(o, want[k]) for k in range(2) for o in got[k])
 
 
+@pytest.fixture(scope="module")
+def impatient(tmp_path_factory):
+    """The kernels with a wait that runs out (tests/native/pages_timeout.cu)."""
+    import ctypes
+    import os
+    import shutil
+    import subprocess
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("nvcc not available")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    so = str(tmp_path_factory.mktemp("native") / "pages_timeout.so")
+    subprocess.check_call([nvcc, "-std=c++17", "-O3", "--expt-relaxed-constexpr", "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompiler", "-fPIC",
+                           "-I", os.path.join(root, "include"), "-I", os.path.join(root, "sbvr-cpu-arm_b200", "csrc"),
+                           "-o", so, os.path.join(root, "tests", "native", "pages_timeout.cu")])
+    from sbvr import _lib
+    lib = ctypes.CDLL(so)
+    lib.sbvr_pages_attention_f16.argtypes = _lib.lib.sbvr_pages_attention_f16.argtypes
+    return lib
+
+
+# warps and barriers by their numbers: 128 rows: 0-3 weights, 4 MMAs, 5 K, 6 V; [2] K, V there, [2] K, V read, [2] scores, weights, outputs there, -, V to be
+# looked through, queries.  256 rows: 0-7, 8, 9, 10; [5] each of the first four, [4] of the next three.
+PROMPT, SHARED = (2, 2, 200, 150, 100, 8, 2, 32), (1, 40, 3000, 20, 1, 32, 8, 64)
+
+
+@pytest.mark.parametrize("case,warp,bar,parity", [
+    (PROMPT, 4, 0, 0), (PROMPT, 4, 3, 0), (PROMPT, 4, 10, 0), (PROMPT, 4, 16, 0), (PROMPT, 5, 4, 0), (PROMPT, 6, 7, 0), (PROMPT, 6, 15, 0), (PROMPT, 0, 8, 1),
+    (PROMPT, 3, 9, 0), (PROMPT, 2, 12, 0),
+    (SHARED, 8, 1, 0), (SHARED, 8, 7, 0), (SHARED, 8, 26, 0), (SHARED, 8, 35, 0), (SHARED, 9, 10, 0), (SHARED, 10, 16, 0), (SHARED, 1, 20, 0), (SHARED, 6, 23, 1),
+    (SHARED, 4, 30, 0)])
+def test_a_wait_that_runs_out_costs_time_and_no_result(impatient, case, warp, bar, parity):
+    import ctypes
+
+    from sbvr import _lib
+    groups, per, shared, own, tps, nh, nkv, page = case
+    c, q, pos, slots, starts = batch(*case, seed=31)
+    sl, common, n = ints(slots), c.common(slots, starts), groups * per
+    need = ctypes.c_size_t(0)
+    cache = ctypes.cast(c._at, ctypes.POINTER(_lib.Pages))
+    _lib.check(_lib.lib.sbvr_pages_attention_scratch_bytes(cache, n, tps, nh, groups, ctypes.byref(need)))
+    scratch = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    assert impatient.pages_wait_that_runs_out(warp, bar, parity) == 0
+    rc = impatient.sbvr_pages_attention_f16(cache, 0, q.data_ptr(), nh * D, sl.data_ptr(), pos.data_ptr(), starts.data_ptr(), common.data_ptr(), groups,
+                                            out.data_ptr(), scratch.data_ptr(), need.value, n, tps, nh, D ** -0.5, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    close(out, attention(c, 0, q, pos, slots, nh), shared + own)
+
+
 def test_refusals():
     from sbvr import _lib
     c, q, pos, slots, starts = batch(1, 4, 64, 20, 1, 8, 2, 16, seed=23)

@@ -42,11 +42,12 @@ def test_arguments_that_are_refused():
     assert lib.sbvr_pages_fork(ctypes.byref(describe(max_seqs=2000)), x, x, 1025, 1, None) == -7
     assert lib.sbvr_pages_common(c, None, 1, None, 1, x, None) == -1 and lib.sbvr_pages_common(c, None, 0, x, 1, x, None) == -1
     rope = lambda **k: lib.sbvr_pages_rope_append_f16(c, *[k.get(n, d) for n, d in (       # noqa: E731
-        ("layer", 0), ("qkv", x), ("pos", x), ("inv", x), ("s", 1.0), ("slots", None), ("seqs", 1), ("tps", 1), ("nh", 4), ("q", x))], None)
+        ("layer", 0), ("qkv", x), ("pos", x), ("inv", x), ("s", 1.0), ("slots", None), ("seqs", 1), ("tps", 1), ("nh", 4), ("q", 2 * x))], None)
     assert rope(layer=2) == -1 and rope(layer=-1) == -1 and rope(seqs=0) == -1 and rope(seqs=5) == -1 and rope(qkv=x + 8) == -3 and rope(q=None) == -1
     assert rope(seqs=1 << 20, tps=1 << 12, slots=x) == -7
+    assert rope(q=x) == -1 and rope(q=x + 2032) == -1 and rope(q=x - 1008) == -1      # rows in one another's place
     att = lambda **k: lib.sbvr_pages_attention_f16(c, *[k.get(n, d) for n, d in (          # noqa: E731
-        ("layer", 0), ("q", x), ("pitch", 512), ("slots", None), ("pos", x), ("starts", None), ("shared", None), ("groups", 0), ("out", x), ("scratch", None),
+        ("layer", 0), ("q", x), ("pitch", 512), ("slots", None), ("pos", x), ("starts", None), ("shared", None), ("groups", 0), ("out", 2 * x), ("scratch", None),
         ("bytes", 0), ("seqs", 1), ("tps", 1), ("nh", 4), ("scale", 1.0))], None)
     for bad in (dict(layer=2), dict(q=None), dict(pos=None), dict(out=None), dict(seqs=0), dict(tps=0), dict(nh=3), dict(nh=0), dict(groups=-1), dict(groups=1),
                 dict(groups=2, starts=x, shared=x), dict(pitch=504), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
@@ -54,6 +55,7 @@ def test_arguments_that_are_refused():
         assert att(**bad) == -1, bad
     assert att(q=x + 8) == -3 and att(pitch=513) == -3 and att(out=x + 4) == -3 and att(scratch=x + 4) == -3
     assert att(seqs=1 << 20, tps=1 << 10, slots=x) == -7
+    assert att(out=x) == -1 and att(out=x + 1008) == -1 and att(q=2 * x + 1008) == -1
 
 
 @pytest.mark.parametrize("kw", [dict(head_dim=64), dict(page_size=48), dict(pages=0), dict(layers=0), dict(max_seqs=0), dict(max_seqs=70000), dict(pages=2 ** 26),

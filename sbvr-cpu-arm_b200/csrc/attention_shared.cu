@@ -7,13 +7,20 @@
 //   output   O[128 rows, 128 dims] += weights . V, weights from tensor memory, V as it lies in the cache
 // The reference of a row is the largest score it has met, but follows it only when that has grown by more than 2^5: then its sums are scaled.
 //
-// Shared keys: the tiles of all blocks in one list, cut into equal shares, one per CTA; a share may end one block and begin the next.
-// Prompts: a CTA per block and part of its tiles, longest blocks first.
+// Shared keys: every block's tiles are cut into pieces, one per CTA where that fits (attention_pages.cuh).  Prompts: a CTA per block, or per part of its
+// tiles where blocks are few, longest blocks first.
 //
 // Warps: four per 128 rows form weights; one issues the MMAs (one lane); two bring K and V, boxes of a page by TMA (places past the last page: a box
-// behind the end, which TMA fills with zeros).  Blocks of 128 rows: two CTAs per SM.  256 rows (two sets of S and O in tensor memory, a tile of K and V
-// for both): one.  Every wait is bounded; a CTA in which one runs out, or among whose keys values are not finite that only some rows attend to, multiplies its
-// rows out without the tensor cores.
+// behind the end, which TMA fills with zeros).  The roles run through the pieces of a CTA by mbarriers alone.  Blocks of 128 rows: two CTAs per SM.  256 rows
+// (two sets of S and O in tensor memory, a tile of K and V for both): one; it is taken where a group has more than 128 rows on average, to read its keys
+// half as often: 128 sequences of 4 heads on 65536 keys 192 us, in blocks of 128 201.  Prompts take 128 rows throughout: uneven lengths leave less idle
+// (8 x 300 tokens on 4001: 151 us, with 256 164).  Every wait is bounded; a CTA in which one runs out, or among whose keys values are not finite that only
+// some rows attend to, multiplies its rows out without the tensor cores.
+//
+// What bounds it.  Few rows: bytes (32 KB a tile, 6.5 TB/s), behind 5 us of prologue (pieces, queries, the first keys) and 2 of sums.  Many rows: the chain from
+// scores to weights to outputs of a tile, about 1900 cycles for 256 rows, in which the tensor pipe works 1280 (768 for S, whose 64 columns read the queries
+// from shared memory again for each tile, 512 for O) and the units for exponentials 1024.  Without exponentials a launch takes as long, with an
+// eighth of the MMAs a tenth less.  Tried without gain: a polynomial for some exponentials, two warps per 32 rows, a warp each for the MMAs of S and of O.
 #include <cuda.h>
 
 #include <climits>
@@ -69,30 +76,13 @@ __device__ __forceinline__ void aq_st16(uint32_t taddr, const uint32_t* a) {
                  "r"(a[14]), "r"(a[15])
                  : "memory");
 }
-// 2^x of two numbers by multiplications and additions: the whole part by the exponent, the rest, at most a half, by a polynomial of degree 4 fitted to the
-// smallest largest relative error (2.7e-6, a 180th of fp16's half step).  Below 2^-125 it stays at that; NaN stays NaN.
-__device__ __forceinline__ float2 as_exp2_pair(float2 x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.0f));
-    const float2 big = make_float2(12582912.0f, 12582912.0f);           // 1.5 * 2^23: rounds to a whole number
-    const float2 t = as_add2(x, big), n = as_add2(t, make_float2(-12582912.0f, -12582912.0f)), f = as_fma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 y = as_fma2(make_float2(9.570101276040077e-3f, 9.570101276040077e-3f), f, make_float2(5.591785907745361e-2f, 5.591785907745361e-2f));
-    y = as_fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    y = as_fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    y = as_fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    const float2 s = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-    return as_fma2(y, s, make_float2(0.0f, 0.0f));
-}
-// weights 2^(s sl2 - base) of 32 scores as fp16, their sums added to `sum`.  AS_POLY of sixteen pairs go the way above, which leaves the units for
-// exponentials (4 lanes a cycle and scheduler) that many fewer.
-constexpr int AS_POLY = 0;
+// weights 2^(s sl2 - base) of 32 scores as fp16, their sums added to `sum`
 __device__ __forceinline__ void as_weights32(const uint32_t* u, float sl2, float base, uint32_t* w, float2 (&sum)[2]) {
     const float2 a = make_float2(sl2, sl2), c = make_float2(-base, -base);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         float2 x = as_fma2(make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])), a, c);
-        if ((e * AS_POLY) % 16 + AS_POLY > 15) x = as_exp2_pair(x);
-        else x.x = ao_exp2(x.x), x.y = ao_exp2(x.y);
+        x.x = ao_exp2(x.x), x.y = ao_exp2(x.y);
         sum[e & 1] = as_add2(sum[e & 1], x);
         const __half2 h = __floats2half2_rn(x.x, x.y);
         w[e] = *reinterpret_cast<const uint32_t*>(&h);
@@ -592,8 +582,8 @@ int launch_attention_shared(const AoParams& p, bool prompt, int nsplit, int grid
     int rc = ts_map_2d(&kmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, p.k, map_rows, AO_D, AO_D * 2, box, 64);
     if (!rc) rc = ts_map_2d(&vmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, p.v, map_rows, AO_D, AO_D * 2, box, 64);
     if (rc) return rc;
-    if (p.rows == 128) return prompt ? launch_shape<1, true>(p, kmap, vmap, nsplit, grid, st) : launch_shape<1, false>(p, kmap, vmap, nsplit, grid, st);
-    return prompt ? launch_shape<2, true>(p, kmap, vmap, nsplit, grid, st) : launch_shape<2, false>(p, kmap, vmap, nsplit, grid, st);
+    if (prompt) return launch_shape<1, true>(p, kmap, vmap, nsplit, grid, st);
+    return p.rows == 128 ? launch_shape<1, false>(p, kmap, vmap, nsplit, grid, st) : launch_shape<2, false>(p, kmap, vmap, nsplit, grid, st);
 }
 
 }  // namespace sbvr

@@ -125,7 +125,7 @@ class PagedCache:
     # ------------------------------------------------------------------ a layer's tokens
     def rope_append(self, layer: int, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, slots: Slots = None, scaling: float = 1.0,
                     q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """qkv [tokens, (n_heads + 2 n_kv) * 128], as many tokens for every slot, at `positions` (below 0: a place of the batch that holds no
+        """qkv [tokens, (n_heads + 2 n_kv) * 128], as many tokens for every slot of `slots` (None: of all, in order), at `positions` (below 0: a place of the batch that holds no
         token).  Returns the rotated queries; k and v go to the slots' pages."""
         return _lib.native.pages_rope_append(self._at, self.device.index, layer, qkv, positions, inv_freq, scaling,
                                              None if slots is None else self._slots(slots, twice=True), self.max_seqs, q_out)

@@ -585,35 +585,39 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
         need = [-(-(L + n + max_new_tokens - 1) // page) for n in lens]
         if B > cache.max_seqs or max(need) > cache.max_pages or whole + sum(n - whole for n in need) > cache.pages:
             raise ValueError("sequences beyond the cache in pages that this model was given")
+        if bool(cache.lengths[:B].any()):
+            raise ValueError(f"slots 0 .. {B - 1} of the cache hold sequences already")
         out = torch.empty((B, max_new_tokens), dtype=torch.int32, device=self.device)
-        if L:                                      # the common beginning, once, in slot 0
-            b = self._act_paged(L, 1, 1)
-            b.ids.copy_(prefix_ids.reshape(-1).to(torch.int32))
-            b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], L, tokens_per_seq=L))
-            b.extra["paged"]["shared"].zero_()
-            self._forward_rows(b, L, last_only=True)
-            if B > 1:
-                cache.fork([0] * (B - 1), list(range(1, B)))
-        d = self._act_paged(B, B, B)
-        d.extra["paged"]["shared"].copy_(cache.common(d.extra["paged"]["slots"], d.extra["paged"]["starts"]))
-        b = self._act_paged(B * P, B, B) if P > 1 else d
-        b.ids.copy_(prompt_ids.reshape(-1).to(torch.int32))
-        b.extra["paged"]["shared"].copy_(d.extra["paged"]["shared"])
-        b.extra["last"] = torch.tensor([i * P + n - 1 for i, n in enumerate(lens)], device=self.device) if P > 1 else None
-        b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], torch.tensor(lens, dtype=torch.int32, device=self.device), tokens_per_seq=P))
-        self._forward_rows(b, P, last_only=True)
-        out[:, 0] = b.next_ids
-        d.ids.copy_(b.next_ids)
-        if max_new_tokens > 1:
-            if use_graph and (self._shared_graph is None or self._shared_graph[0] != B):
-                self._shared_graph = (B, self._capture_shared(d))
-            for i in range(1, max_new_tokens):
-                if use_graph:
-                    self._shared_graph[1].replay()
-                else:
-                    self._shared_step(d)
-                out[:, i] = d.ids
-        cache.free(d.extra["paged"]["slots"])
+        try:
+            if L:                                      # the common beginning, once, in slot 0
+                b = self._act_paged(L, 1, 1)
+                b.ids.copy_(prefix_ids.reshape(-1).to(torch.int32))
+                b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], L, tokens_per_seq=L))
+                b.extra["paged"]["shared"].zero_()
+                self._forward_rows(b, L, last_only=True)
+                if B > 1:
+                    cache.fork([0] * (B - 1), list(range(1, B)))
+            d = self._act_paged(B, B, B)
+            d.extra["paged"]["shared"].copy_(cache.common(d.extra["paged"]["slots"], d.extra["paged"]["starts"]))
+            b = self._act_paged(B * P, B, B) if P > 1 else d
+            b.ids.copy_(prompt_ids.reshape(-1).to(torch.int32))
+            b.extra["paged"]["shared"].copy_(d.extra["paged"]["shared"])
+            b.extra["last"] = torch.tensor([i * P + n - 1 for i, n in enumerate(lens)], device=self.device) if P > 1 else None
+            b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], torch.tensor(lens, dtype=torch.int32, device=self.device), tokens_per_seq=P))
+            self._forward_rows(b, P, last_only=True)
+            out[:, 0] = b.next_ids
+            d.ids.copy_(b.next_ids)
+            if max_new_tokens > 1:
+                if use_graph and (self._shared_graph is None or self._shared_graph[0] != B):
+                    self._shared_graph = (B, self._capture_shared(d))
+                for i in range(1, max_new_tokens):
+                    if use_graph:
+                        self._shared_graph[1].replay()
+                    else:
+                        self._shared_step(d)
+                    out[:, i] = d.ids
+        finally:
+            cache.free(list(range(B)))
         self._check()
         cache.check()
         return out

@@ -408,6 +408,37 @@ def test_two_calls_at_once():
     assert all(torch.equal(o, want[k]) for k in range(2) for o in got[k])
 
 
+@pytest.mark.parametrize("case", [(1, 40, 700, 20, 1, 32, 8, 64), (1, 5, 200, 20, 1, 8, 2, 16), (1, 2, 200, 150, 100, 8, 2, 32), (1, 4, 300, 40, 6, 8, 2, 16)])
+@pytest.mark.parametrize("entry", [-1, 10 ** 6])
+def test_entries_that_name_no_page(case, entry):
+    """Read as keys and values of zeros, and said; what does not read them is what it was."""
+    c, q, pos, slots, starts = batch(*case, seed=41)
+    groups, per, shared, own, tps, nh, nkv, page = case
+    common = c.common(slots, starts)
+    c.check()
+    last = slots[per - 1]
+    k = int(c.lengths[last] - 1) // page
+    kept = c.table.clone()
+    c.table[last, k] = entry                                   # a page of the last sequence's own
+    c.table[slots[0], 1] = entry                               # one that is shared, by its first sequence's row
+    out = c.attention(0, q, pos, ints(slots), group_starts=starts, shared=common)
+    with pytest.raises(RuntimeError, match="no page"):
+        c.check()
+    c.table.copy_(kept)
+    free = int((c.refs == 0).nonzero()[0])
+    c.pool[:, :, free] = 0
+    c.table[last, k] = free
+    for s in (slots if tps * (nh // nkv) < 64 and _shares(c, case) else slots[:1]):
+        c.table[s, 1] = free
+    close(out, attention(c, 0, q, pos, slots, nh), shared + own)
+
+
+def _shares(c, case):
+    """Whether a call reads the first sequence's pages for all of them: where that can save 2 MB (csrc/attention_pages.cu)."""
+    groups, per, shared, own, tps, nh, nkv, page = case
+    return (per - 1) * groups * c.max_pages * page * nkv * 512 > 2 << 20
+
+
 @pytest.fixture(scope="module")
 def impatient(tmp_path_factory):
     """The kernels with a wait that runs out (tests/native/pages_timeout.cu)."""
@@ -535,4 +566,9 @@ def test_generate_shared_refuses_what_does_not_fit():
             m.generate_shared(*args)
     with pytest.raises(ValueError):
         m.generate_shared(ids[0], ids, 2, prompt_lengths=[5, 0])
+    assert m.generate_shared(ids[0], ids, 2).shape == (2, 2)
+    m.pages.reserve([1], 3)
+    with pytest.raises(ValueError, match="already"):
+        m.generate_shared(ids[0], ids, 2)
+    m.pages.free([1])
     assert m.generate_shared(ids[0], ids, 2).shape == (2, 2)

@@ -120,10 +120,10 @@ __global__ void __launch_bounds__(128) pages_free_kernel(const PgCache c, const 
 }
 
 // ---------------------------------------------------------------------------------------------
-// reserve: one block.  scratch: [verdict][need prefix sums, n + 1][free pages].  More than PG_POSITIONS positions are written by a launch of their own behind
+// reserve: one block.  scratch: [4: verdict][two words per slot][free pages].  More than PG_POSITIONS positions are written by a launch of their own behind
 // it (64 slots x 4000 by the one block: 60 us).
 // ---------------------------------------------------------------------------------------------
-constexpr int PG_POSITIONS = 8192;
+constexpr int PG_POSITIONS = 8192, PG_SHARED = 2048;
 
 __global__ void __launch_bounds__(256) pages_positions_kernel(const PgCache c, const int* slots, const int* tokens, int each, int* positions, int tps) {
     pdl_launch_dependents();
@@ -141,8 +141,10 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache
     pdl_launch_dependents();
     pdl_wait();
     int fault = pg_slots_ok(c, slots, n, seen) ? 0 : SBVR_PAGES_BAD_SLOT;
-    int* first = c.scratch + 4;                    // [n + 1]
-    int* list = first + c.max_seqs + 4;
+    // what every slot needs, summed up [n + 1], and the table's entry of its first new page [n]: in shared memory for up to PG_SHARED slots
+    int* first = n <= PG_SHARED ? reinterpret_cast<int*>(seen + (c.max_seqs + 31) / 32) : c.scratch + 4;
+    int* entry = n <= PG_SHARED ? first + n + 1 : c.scratch + 4 + c.max_seqs + 4;
+    int* list = c.scratch + 4 + 2 * (c.max_seqs + 4);
     int sum = 0;
     for (int base = 0; base < n; base += PG_THREADS) {
         const int i = base + threadIdx.x;
@@ -155,7 +157,10 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache
         }
         int total;
         const int at = sum + pg_scan(sc, need, &total);
-        if (i < n) first[i] = at;
+        if (i < n) {
+            first[i] = at;
+            if (!fault) entry[i] = pg_slot(slots, i) * c.max_pages + pg_pages_of(c, c.lengths[pg_slot(slots, i)]);
+        }
         // (needs are bounded by n * max_pages, which the host keeps below 2^31)
         sum += total;
         fault |= __syncthreads_or(bad & SBVR_PAGES_BAD_SLOT) ? SBVR_PAGES_BAD_SLOT : 0;
@@ -179,8 +184,8 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache
             if (first[mid] <= j) lo = mid;
             else hi = mid;
         }
-        const int slot = pg_slot(slots, lo), p = list[j];
-        c.table[(size_t)slot * c.max_pages + pg_pages_of(c, c.lengths[slot]) + (j - first[lo])] = p;
+        const int p = list[j];
+        c.table[entry[lo] + (j - first[lo])] = p;
         c.refs[p] = 1;
     }
     if (positions) {
@@ -586,7 +591,7 @@ int sbvr_pages_reserve(const sbvr_pages_t* cache, const int* slots, const int* t
     if (positions && (long long)n * tokens_per_seq > INT_MAX / 2) return SBVR_ERR_UNSUPPORTED;
     const bool many = positions && (long long)n * tokens_per_seq > PG_POSITIONS;
     if (many && n > 65535) return SBVR_ERR_UNSUPPORTED;
-    SBVR_CUDA_TRY(launch_pdl(pages_reserve_kernel, dim3(1), dim3(PG_THREADS), seen_bytes(c), reinterpret_cast<cudaStream_t>(stream), c, slots, tokens,
+    SBVR_CUDA_TRY(launch_pdl(pages_reserve_kernel, dim3(1), dim3(PG_THREADS), seen_bytes(c) + (n <= PG_SHARED ? (2 * (size_t)n + 1) * 4 : 0), reinterpret_cast<cudaStream_t>(stream), c, slots, tokens,
                              tokens_each, n, many ? nullptr : positions, tokens_per_seq));
     if (many)
         SBVR_CUDA_TRY(launch_pdl(pages_positions_kernel, dim3((unsigned)std::min((tokens_per_seq + 1023) / 1024, 64), (unsigned)n), dim3(256), 0,

@@ -5,7 +5,8 @@
 //   scores   S[128 rows, 64 keys] = q . k, both from shared memory (128-byte swizzle), fp32 in tensor memory
 //   weights  a thread per row: 2^(s - reference + 10) in fp32, rounded to fp16 once, stored over S
 //   output   O[128 rows, 128 dims] += weights . V, weights from tensor memory, V as it lies in the cache
-// The reference of a row is the largest score it has met, but follows it only when that has grown by more than 2^5: then its sums are scaled.
+// The reference of a row is the largest score it has met, but follows it only when the weights of half a tile, 2^10 each for a score like the reference, add up
+// to more than 2^15: then its sums are scaled.  Every weight that is kept is at most that, which fp16 holds.
 //
 // Shared keys: every block's tiles are cut into pieces, one per CTA where that fits (attention_pages.cuh).  Prompts: a CTA per block, or per part of its
 // tiles where blocks are few, longest blocks first.
@@ -13,8 +14,8 @@
 // Warps: four per 128 rows form weights; one issues the MMAs (one lane); two bring K and V, boxes of a page by TMA (places past the last page: a box
 // behind the end, which TMA fills with zeros).  The roles run through the pieces of a CTA by mbarriers alone.  Blocks of 128 rows: two CTAs per SM.  256 rows
 // (two sets of S and O in tensor memory, a tile of K and V for both): one; it is taken where a group has more than 128 rows on average, to read its keys
-// half as often: 128 sequences of 4 heads on 65536 keys 192 us, in blocks of 128 201.  Prompts take 128 rows throughout: uneven lengths leave less idle
-// (8 x 300 tokens on 4001: 151 us, with 256 164).  Every wait is bounded; a CTA in which one runs out, or among whose keys values are not finite that only
+// half as often: 128 sequences of 4 heads on 65536 keys, calls back to back for a second, 220 us, in blocks of 128 225.  Prompts take 128 rows throughout:
+// uneven lengths leave less idle (8 x 300 tokens on 4001: 137 us; an earlier form 151, with 256 rows 164).  Every wait is bounded; a CTA in which one runs out, or among whose keys values are not finite that only
 // some rows attend to, multiplies its rows out without the tensor cores.
 //
 // What bounds it.  Few rows: bytes (32 KB a tile, 6.5 TB/s), behind 5 us of prologue (pieces, queries, the first keys) and 2 of sums.  Many rows: the chain from
@@ -68,13 +69,6 @@ __device__ __forceinline__ float as_top32(const uint32_t* u) {
 #pragma unroll
     for (int e = 4; e < 32; e += 2) m[(e >> 1) & 3] = as_max3(m[(e >> 1) & 3], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
     return as_max3(fmaxf(m[0], m[1]), m[2], m[3]);
-}
-// sixteen columns of tensor memory
-__device__ __forceinline__ void aq_st16(uint32_t taddr, const uint32_t* a) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(a[0]), "r"(a[1]),
-                 "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]), "r"(a[8]), "r"(a[9]), "r"(a[10]), "r"(a[11]), "r"(a[12]), "r"(a[13]),
-                 "r"(a[14]), "r"(a[15])
-                 : "memory");
 }
 // weights 2^(s sl2 - base) of 32 scores as fp16, their sums added to `sum`
 __device__ __forceinline__ void as_weights32(const uint32_t* u, float sl2, float base, uint32_t* w, float2 (&sum)[2]) {
@@ -430,11 +424,12 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
             const int wmin = __reduce_min_sync(0xffffffffu, lim < 0 ? 0x7fffffff : lim);        // (no rows: anything finite)
             const bool idle = !__any_sync(0xffffffffu, lim > 0);
             const float sl2 = p.sl2;
-            // Half a tile at a time, the next half on its way.  Weights are formed with the reference there is, and once more where a score turns out too
-            // large for it: nothing waits for the largest score.  References are whole numbers (of scores times sl2), so that what was formed with the
-            // last one is scaled by a power of two.
+            // Half a tile at a time, the next half on its way.  Weights are formed with the reference there is, and once more, from scores that still stand in
+            // tensor memory, where a half's sum turns out too large for it: nothing waits for the largest score.  What a wait or a vote takes is
+            // asked for before the work that hides it.  References are whole numbers (of scores times sl2): what was summed up with the last one is
+            // scaled by a power of two.
             float ref = -INFINITY, sum = 0.0f;
-            uint32_t u[2][32], w[2][16];
+            uint32_t u[2][32], w[32];
             bool ahead = false;                                  // the first half is on its way
             for (int i = 0; i < cnt; ++i) {
                 const int m = mr + i, b = m & 1, key0 = (s.ta + i) * AS_KEYS;
@@ -447,64 +442,62 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                 }
                 ahead = false;
                 if (!idle) {
+                    const bool ends = key0 + AS_KEYS > wmin;     // some row's keys end inside or before this tile
+                    auto hide = [&](int h) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        aq_ld_wait(u[h]);
-                        if (h == 0) {
-                            aq_ld32(mine + b * 64 + 32, u[1]);
-                        } else if (i + 1 < cnt) {
-                            ahead = __all_sync(0xffffffffu, mbar_test(s_full + 2 * r + (b ^ 1), (uint32_t)((m + 1) >> 1) & 1u));
-                            if (ahead) {
-                                aq_fence_after();
-                                aq_ld32(mine + (b ^ 1) * 64, u[0]);
-                            }
-                        }
-                        if (key0 + 32 * h + 32 > wmin) {         // some row's keys end inside or before these
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (key0 + 32 * h + e >= lim) u[h][e] = 0xff800000u;
-                        }
-                        float2 part[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-                        as_weights32(u[h], sl2, (ref == -INFINITY ? 0.0f : ref) - AO_LIFT, w[h], part);
-                        float all = (part[0].x + part[1].x) + (part[0].y + part[1].y);
-                        if (__any_sync(0xffffffffu, all > 32768.0f || (ref == -INFINITY && key0 + 32 * h < lim))) {
-                            const float now = fmaxf(ref, ceilf(as_top32(u[h]) * sl2)), corr = ref == -INFINITY ? 0.0f : ao_exp2(ref - now);
-                            ref = now;
-                            sum *= corr;
-                            if (h) {
-                                const __half2 c2 = __float2half2_rn(corr);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[0][e]), c2);
-                                    w[0][e] = *reinterpret_cast<const uint32_t*>(&x);
-                                }
-                                aq_st16(mine + b * 64, w[0]);
-                            }
-                            if (i > 0) {
-                                if (!mbar_wait_async(o_done + 2 * r + (b ^ 1), (uint32_t)((m - 1) >> 1) & 1u)) ok = false;
-                                ok = __all_sync(0xffffffffu, ok);
-                                if (!ok) break;
-                                aq_fence_after();
-#pragma unroll 1
-                                for (int c = 0; c < 8; ++c) {
-                                    uint32_t lo[8], hi[8];
-                                    ts_ld16_issue(mine + 128 + c * 16, lo, hi);
-                                    ts_wait_ld(lo), ts_wait_ld(hi);
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e)
-                                        lo[e] = __float_as_uint(__uint_as_float(lo[e]) * corr), hi[e] = __float_as_uint(__uint_as_float(hi[e]) * corr);
-                                    ts_st8(mine + 128 + c * 16, lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]);
-                                    ts_st8(mine + 128 + c * 16 + 8, hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]);
-                                }
-                            }
-                            part[0] = part[1] = make_float2(0.0f, 0.0f);
-                            as_weights32(u[h], sl2, (ref == -INFINITY ? 0.0f : ref) - AO_LIFT, w[h], part);
-                            all = (part[0].x + part[1].x) + (part[0].y + part[1].y);
-                        }
-                        sum += all;
-                        aq_st16(mine + b * 64 + 16 * h, w[h]);   // (over scores that are in registers)
+                        for (int e = 0; e < 32; ++e)
+                            if (key0 + 32 * h + e >= lim) u[h][e] = 0xff800000u;
+                    };
+                    aq_ld_wait(u[0]);
+                    aq_ld32(mine + b * 64 + 32, u[1]);
+                    const bool soon = i + 1 < cnt && mbar_test(s_full + 2 * r + (b ^ 1), (uint32_t)((m + 1) >> 1) & 1u);
+                    if (ends) hide(0);
+                    float2 p0[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}}, p1[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+                    const float base = (ref == -INFINITY ? 0.0f : ref) - AO_LIFT;
+                    as_weights32(u[0], sl2, base, w, p0);
+                    aq_ld_wait(u[1]);
+                    ahead = __all_sync(0xffffffffu, soon);
+                    if (ahead) {
+                        aq_fence_after();
+                        aq_ld32(mine + (b ^ 1) * 64, u[0]);
                     }
-                    if (!ok) break;
+                    if (ends) hide(1);
+                    as_weights32(u[1], sl2, base, w + 16, p1);
+                    float a0 = (p0[0].x + p0[1].x) + (p0[0].y + p0[1].y), a1 = (p1[0].x + p1[1].x) + (p1[0].y + p1[1].y);
+                    if (__any_sync(0xffffffffu, fmaxf(a0, a1) > 32768.0f || (ref == -INFINITY && key0 < lim))) {
+                        aq_ld_wait(u[0]);                        // (the next tile's first half is asked for again)
+                        ahead = false;
+                        aq_ld32(mine + b * 64, u[0]);
+                        aq_ld_wait(u[0]);
+                        if (ends) hide(0);
+                        const float now = fmaxf(ref, ceilf(fmaxf(as_top32(u[0]), as_top32(u[1])) * sl2)), corr = ref == -INFINITY ? 0.0f : ao_exp2(ref - now);
+                        ref = now;
+                        sum *= corr;
+                        if (i > 0) {
+                            if (!mbar_wait_async(o_done + 2 * r + (b ^ 1), (uint32_t)((m - 1) >> 1) & 1u)) ok = false;
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            aq_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < 8; ++c) {
+                                uint32_t lo[8], hi[8];
+                                ts_ld16_issue(mine + 128 + c * 16, lo, hi);
+                                ts_wait_ld(lo), ts_wait_ld(hi);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    lo[e] = __float_as_uint(__uint_as_float(lo[e]) * corr), hi[e] = __float_as_uint(__uint_as_float(hi[e]) * corr);
+                                ts_st8(mine + 128 + c * 16, lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]);
+                                ts_st8(mine + 128 + c * 16 + 8, hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]);
+                            }
+                        }
+                        p0[0] = p0[1] = make_float2(0.0f, 0.0f);
+                        const float moved = (ref == -INFINITY ? 0.0f : ref) - AO_LIFT;
+                        as_weights32(u[0], sl2, moved, w, p0);
+                        as_weights32(u[1], sl2, moved, w + 16, p0);
+                        a0 = (p0[0].x + p0[1].x) + (p0[0].y + p0[1].y), a1 = 0.0f;
+                    }
+                    sum += a0 + a1;
+                    aq_st32(mine + b * 64, w);                   // (over scores that are in registers)
                     aq_st_wait();
                 }
                 aq_fence_before();

@@ -561,6 +561,17 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             self._bufs[key] = b
         return b
 
+    def _checked_ids(self, ids: torch.Tensor, lens: Optional[List[int]] = None) -> torch.Tensor:
+        """Token ids as the embedding reads them, int32 on the model's device.  With `lens`, row i of `ids` holds lens[i] tokens; the places behind
+        them may hold anything (-1, a pad id) and become 0.  Every token has to be a row of the table: the kernel does not look.  Waits for the GPU."""
+        ids = ids.to(self.device)
+        if lens is not None:
+            held = torch.arange(ids.shape[1], device=self.device) < torch.tensor(lens, device=self.device)[:, None]
+            ids = torch.where(held, ids, torch.zeros_like(ids))
+        if bool(((ids < 0) | (ids >= self.embed_tokens.shape[0])).any()):
+            raise ValueError("token ids outside the vocabulary")
+        return ids.reshape(-1).to(torch.int32)
+
     def _shared_step(self, b: _Buffers):
         """One decode step of all sequences: room for a token each, the step, its tokens as the next one's."""
         b.positions.copy_(self.pages.reserve(b.extra["paged"]["slots"], 1, tokens_per_seq=1))
@@ -571,8 +582,8 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
     def generate_shared(self, prefix_ids: torch.Tensor, prompt_ids: torch.Tensor, max_new_tokens: int,
                         prompt_lengths: Optional[torch.Tensor] = None, use_graph: bool = True) -> torch.Tensor:
         """Greedy generation for prompts that begin alike: `prefix_ids` [L] is run once and held once, every row of `prompt_ids` [B, P] (its first
-        `prompt_lengths[i]` >= 1 tokens; all of them by default) goes on from it.  Needs `attach_pages`; uses its slots 0 .. B - 1, which hold nothing
-        before and after.  Returns [B, max_new_tokens] int32."""
+        `prompt_lengths[i]` >= 1 tokens, whatever stands behind them; all of them by default) goes on from it.  Needs `attach_pages`; uses its slots
+        0 .. B - 1, which hold nothing before and after.  Returns [B, max_new_tokens] int32."""
         cache = self.pages
         if cache is None:
             raise RuntimeError("generate_shared needs a cache in pages: call attach_pages first")
@@ -587,11 +598,12 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             raise ValueError("sequences beyond the cache in pages that this model was given")
         if bool(cache.lengths[:B].any()):
             raise ValueError(f"slots 0 .. {B - 1} of the cache hold sequences already")
+        prefix, prompts = self._checked_ids(prefix_ids), self._checked_ids(prompt_ids, lens)
         out = torch.empty((B, max_new_tokens), dtype=torch.int32, device=self.device)
         try:
             if L:                                      # the common beginning, once, in slot 0
                 b = self._act_paged(L, 1, 1)
-                b.ids.copy_(prefix_ids.reshape(-1).to(torch.int32))
+                b.ids.copy_(prefix)
                 b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], L, tokens_per_seq=L))
                 b.extra["paged"]["shared"].zero_()
                 self._forward_rows(b, L, last_only=True)
@@ -600,7 +612,7 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             d = self._act_paged(B, B, B)
             d.extra["paged"]["shared"].copy_(cache.common(d.extra["paged"]["slots"], d.extra["paged"]["starts"]))
             b = self._act_paged(B * P, B, B) if P > 1 else d
-            b.ids.copy_(prompt_ids.reshape(-1).to(torch.int32))
+            b.ids.copy_(prompts)
             b.extra["paged"]["shared"].copy_(d.extra["paged"]["shared"])
             b.extra["last"] = torch.tensor([i * P + n - 1 for i, n in enumerate(lens)], device=self.device) if P > 1 else None
             b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], torch.tensor(lens, dtype=torch.int32, device=self.device), tokens_per_seq=P))

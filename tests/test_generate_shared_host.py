@@ -1,0 +1,87 @@
+"""`SBVRLlamaForCausalLM.generate_shared` without a GPU: a cache in pages that keeps its books in plain Python (tests/pages_model.py) and a step that only
+records what it is given."""
+import pytest
+import torch
+
+from tests.pages_model import Model
+
+
+class Cache:
+    """What generate_shared uses of models.pages.PagedCache."""
+
+    def __init__(self, pages=60, page_size=16, max_seqs=8, max_pages=40):
+        self.m = Model(pages, page_size, max_seqs, max_pages, torch.zeros(1, 1, pages, 1, page_size, 1))
+        self.pages, self.page_size, self.max_seqs, self.max_pages = pages, page_size, max_seqs, max_pages
+
+    lengths = property(lambda self: torch.tensor(self.m.lengths, dtype=torch.int32))
+    refs = property(lambda self: torch.tensor(self.m.refs, dtype=torch.int32))
+
+    @staticmethod
+    def _list(v, n=None):
+        return v.tolist() if isinstance(v, torch.Tensor) else [v] * n if isinstance(v, int) else list(v)
+
+    def reserve(self, slots, tokens, tokens_per_seq=0):
+        slots = self._list(slots)
+        return torch.tensor(self.m.reserve(slots, self._list(tokens, len(slots)), tokens_per_seq), dtype=torch.int32)
+
+    def free(self, slots):
+        self.m.free(self._list(slots))
+
+    def fork(self, src, dst):
+        assert 1 <= len(dst) <= 1024                           # (of one call of the library)
+        self.m.fork(self._list(src), self._list(dst))
+
+    def common(self, slots, starts):
+        slots, starts = self._list(slots), self._list(starts)
+        return torch.tensor([self.m.common(slots[a:b]) for a, b in zip(starts, starts[1:])], dtype=torch.int32)
+
+    def check(self):
+        bits, self.m.status = self.m.status, 0
+        if bits:
+            raise RuntimeError(f"status {bits}")
+
+
+def model(monkeypatch, cache):
+    """A tiny model whose steps note the ids and positions they are given and answer with the last ids, plus one."""
+    from models.sbvr_llama import LlamaConfig, SBVRLlamaForCausalLM
+    m = SBVRLlamaForCausalLM(LlamaConfig.preset("tiny"), device="cpu", max_batch=8, max_ctx=16)
+    m.embed_tokens = torch.zeros((m.config.vocab_size, 1), dtype=torch.float16)
+    m.pages, m.steps = cache, []
+
+    def step(b, tokens_per_seq, last_only):
+        m.steps.append((b.ids.clone(), b.positions.clone()))
+        b.next_ids.fill_(len(m.steps))
+    monkeypatch.setattr(m, "_forward_rows", step)
+    monkeypatch.setattr(m, "_check", lambda: None)
+    return m
+
+
+@pytest.mark.parametrize("L,P", [(20, 5), (0, 4), (16, 1)])
+def test_places_without_a_token_read_no_row_of_the_embedding(monkeypatch, L, P):
+    """What stands behind a prompt's last token may be anything: -1, -100, an id behind the vocabulary."""
+    m = model(monkeypatch, Cache())
+    V = m.config.vocab_size
+    lens = [P, max(1, P - 2), 1]
+    prompts = torch.arange(3 * P).view(3, P) % V
+    for i, n in enumerate(lens):
+        prompts[i, n:] = torch.tensor([-1, -100, V, 2 ** 40])[:P - n]
+    m.generate_shared(torch.arange(L), prompts, 3, prompt_lengths=lens, use_graph=False)
+    assert len(m.steps) == (L > 0) + 3
+    for ids, _ in m.steps:
+        assert ((ids >= 0) & (ids < V)).all()
+    ids, pos = m.steps[L > 0]
+    for i, n in enumerate(lens):
+        assert torch.equal(ids.view(3, P)[i, :n].long(), prompts[i, :n])
+        assert pos.view(3, P)[i].tolist() == [L + j if j < n else -1 for j in range(P)]
+
+
+@pytest.mark.parametrize("where", ["prefix", "prompt"])
+@pytest.mark.parametrize("bad", [-1, 1024, 2 ** 32])
+def test_ids_outside_the_vocabulary_are_refused(monkeypatch, where, bad):
+    m = model(monkeypatch, Cache())
+    assert m.config.vocab_size == 1024
+    prefix, prompts = torch.arange(20), torch.arange(8).view(2, 4)
+    (prefix if where == "prefix" else prompts.view(-1))[3] = bad
+    with pytest.raises(ValueError, match="vocabulary"):
+        m.generate_shared(prefix, prompts, 2, use_graph=False)
+    assert not m.steps and not m.pages.refs.any()

@@ -572,3 +572,21 @@ def test_generate_shared_refuses_what_does_not_fit():
         m.generate_shared(ids[0], ids, 2)
     m.pages.free([1])
     assert m.generate_shared(ids[0], ids, 2).shape == (2, 2)
+
+
+def test_generate_shared_ignores_what_pads_a_prompt():
+    """Rows padded with -1, -100, the largest id there is, and with ids of the vocabulary: the same tokens."""
+    m = tiny()
+    m.attach_pages(60, 16, max_seqs=8)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    prefix = torch.randint(0, 1024, (37,), device="cuda", generator=g)
+    prompts = torch.randint(0, 1024, (4, 9), device="cuda", generator=g)
+    lens = [9, 1, 4, 8]
+    want = m.generate_shared(prefix, prompts, 5, prompt_lengths=lens)
+    for pad in (-1, -100, 2 ** 31 - 1):
+        padded = prompts.clone()
+        for i, n in enumerate(lens):
+            padded[i, n:] = pad
+        assert torch.equal(m.generate_shared(prefix, padded, 5, prompt_lengths=lens), want)
+        with pytest.raises(ValueError, match="vocabulary"):
+            m.generate_shared(prefix, padded, 5)

@@ -258,20 +258,24 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
         if self.tp_size == 1 and self.tp_group is None:
             return False
         from .comm import SymmetricAllReduce
+        self._drop_graphs()                        # (they hold the block, descriptors and step counter that are replaced here)
         try:
             self._comm = SymmetricAllReduce(self.tp_group, self.device, max_rows, self.config.hidden_size,
                                             2 * self.config.num_hidden_layers)
         except Exception as e:                     # no peer mapping on this machine: NCCL stays
             self._comm_error = repr(e)
             self._comm = None
-        self._graph = None
         return self._comm is not None
 
     def set_pushed_allreduce(self, on: bool) -> None:
         """Decode (up to four rows): whether the row-parallel linears push their results into the ranks' receive areas
         (on by default) or write partials that the one-shot all-reduce kernel then reads over NVLink."""
         self.pushed_allreduce = bool(on)
-        self._graph = None
+        self._drop_graphs()
+
+    def _drop_graphs(self) -> None:
+        """The captured decode steps, on the dense cache and on the one in pages, whose kernels or buffers are about to change."""
+        self._graph = self._shared_graph = None
 
     def _alloc_cache(self):
         c = self.config

@@ -85,3 +85,21 @@ def test_ids_outside_the_vocabulary_are_refused(monkeypatch, where, bad):
     with pytest.raises(ValueError, match="vocabulary"):
         m.generate_shared(prefix, prompts, 2, use_graph=False)
     assert not m.steps and not m.pages.refs.any()
+
+
+def test_what_a_step_runs_on_changes_and_its_graphs_go(monkeypatch):
+    """Graphs hold the addresses and the choice of kernels of the time they were captured at: none outlives a change of the all-reduces."""
+    import models.comm
+    m = model(monkeypatch, Cache())
+    m._graph, m._shared_graph = "dense", (1, "in pages")
+    m.set_pushed_allreduce(False)
+    assert m._graph is None and m._shared_graph is None and m.pushed_allreduce is False
+    for unavailable in (False, True):
+        def comm(*a):
+            if unavailable:
+                raise RuntimeError("no peer mapping")
+            return "block"
+        monkeypatch.setattr(models.comm, "SymmetricAllReduce", comm)
+        m.tp_group, m._graph, m._shared_graph = "group", "dense", (1, "in pages")
+        assert m.enable_fused_allreduce() is not unavailable
+        assert m._graph is None and m._shared_graph is None

@@ -6,7 +6,7 @@
 //   attention_own_kernel       every sequence's own keys (all of them where nothing is shared), joined with those sums
 // Many rows per sequence (prompts): the first kernel takes the rows of one sequence as its blocks and all keys they attend to.
 //
-// A part of a softmax is (m, l, o): o = sum of 2^(s - m) v, l = sum of 2^(s - m) over its keys, s the scores times scale * log2(e), all fp32.
+// A part of a softmax is (m, l, o): o = sum of 2^(s - m + 10) v, l = sum of 2^(s - m + 10) over its keys, s the scores times scale * log2(e), all fp32.
 // Parts join as M = max m, l = sum l 2^(m - M), o = sum o 2^(m - M); a part without keys has m = -inf, l = 0.
 #include <algorithm>
 #include <climits>
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
         float corr[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float x[4] = {s[0][2 * h] * p.sl2, s[0][2 * h + 1] * p.sl2, s[1][2 * h] * p.sl2, s[1][2 * h + 1] * p.sl2};
+            float x[4] = {__fmul_rn(s[0][2 * h], p.sl2), __fmul_rn(s[0][2 * h + 1], p.sl2), __fmul_rn(s[1][2 * h], p.sl2), __fmul_rn(s[1][2 * h + 1], p.sl2)};
             if (key0 + AO_KEYS > least) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -202,12 +202,12 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             top = fmaxf(top, m[h]);
-            const float base = (top == -INFINITY ? 0.0f : top) - AO_LIFT;
+            const float base = top == -INFINITY ? 0.0f : top;
             corr[h] = m[h] == -INFINITY ? 0.0f : ao_exp2(m[h] - top);
             m[h] = top;
             l[h] *= corr[h];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[h][e] = ao_exp2(x[e] - base), l[h] += f[h][e];
+            for (int e = 0; e < 4; ++e) f[h][e] = ao_exp2((x[e] - base) + AO_LIFT), l[h] += f[h][e];
             const __half2 a = __floats2half2_rn(f[h][0], f[h][1]), b = __floats2half2_rn(f[h][2], f[h][3]);
             w[h] = *reinterpret_cast<const uint32_t*>(&a), w[2 + h] = *reinterpret_cast<const uint32_t*>(&b);
         }
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     float* o_s = reinterpret_cast<float*>(ao_smem);                // [warp][16][AO_PITCH]
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        if (t4 == 0) ml_s[warp][g + 8 * h] = make_float2(m[h] == -INFINITY ? m[h] : m[h] - AO_LIFT, l[h]);
+        if (t4 == 0) ml_s[warp][g + 8 * h] = make_float2(m[h], l[h]);
         if (g + 8 * h < nrows) {
 #pragma unroll
             for (int n = 0; n < 16; ++n)

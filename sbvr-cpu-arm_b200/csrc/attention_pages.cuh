@@ -11,8 +11,10 @@ namespace sbvr {
 
 constexpr int AO_D = PG_D;
 // Weights become fp16 for the second product: half a step, 2^-11, of each.  They are multiplied by 2^10 first, so that what is 2^-24 and more of
-// the largest keeps all of its bits; the reference a weight is taken from may lag 2^5 behind the largest: at most 2^15.
-constexpr float AO_LIFT = 10.0f;
+// the largest keeps all of its bits; the reference a weight is taken from may lag 2^5 behind the largest: at most 2^15.  The 2^10 stays in the sums of
+// every part and cancels in the end.  It is added to the difference of score and reference, never to the reference alone: from 2^24 on that loses it, and
+// from 2^26 on fma(score, scale, -reference) keeps more of the largest score than the reference did: weights that fp16 does not hold.
+constexpr float AO_LIFT = 10.0f, AO_LIFTED = 1024.0f;
 
 struct AoParams {
     PgCache c;

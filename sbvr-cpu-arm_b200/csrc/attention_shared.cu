@@ -8,6 +8,8 @@
 // The reference of a row is the largest score it has met, but follows it only when the weights of half a tile, 2^10 each for a score like the reference, add up
 // to more than 2^15: then its sums are scaled.  Every weight that is kept is at most that, which fp16 holds.
 //
+// A reference of 2^22 and more has no room for fractions beside it: such a piece is multiplied out without the tensor cores, weights in fp32.
+//
 // Shared keys: every block's tiles are cut into pieces, one per CTA where that fits (attention_pages.cuh).  Prompts: a CTA per block, or per part of its
 // tiles where blocks are few, longest blocks first.
 //
@@ -200,8 +202,8 @@ __device__ __noinline__ void as_multiply_out(const AoParams& p, const AsSeg& s, 
             for (int i = 0; i < 4; ++i) o[i] = o[i] * corr + e * v[i];
         }
         if (s.place >= 0) {
-            as_store(p, s.place, rows, row, lane, make_float4(o[0], o[1], o[2], o[3]));
-            if (lane == 0) as_store_ml(p, s.place, rows, row, m, l);
+            as_store(p, s.place, rows, row, lane, make_float4(o[0] * AO_LIFTED, o[1] * AO_LIFTED, o[2] * AO_LIFTED, o[3] * AO_LIFTED));
+            if (lane == 0) as_store_ml(p, s.place, rows, row, m, l * AO_LIFTED);
         } else {
             const float inv = 1.0f / l;
             const bool on = l > 0.0f || l != l;
@@ -472,6 +474,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                         if (ends) hide(0);
                         const float now = fmaxf(ref, ceilf(fmaxf(as_top32(u[0]), as_top32(u[1])) * sl2)), corr = ref == -INFINITY ? 0.0f : ao_exp2(ref - now);
                         ref = now;
+                        if (fabsf(ref) >= 4194304.0f && fabsf(ref) < INFINITY) atomicOr(const_cast<int*>(odd_s), 1 << (j & 31));
                         sum *= corr;
                         if (i > 0) {
                             if (!mbar_wait_async(o_done + 2 * r + (b ^ 1), (uint32_t)((m - 1) >> 1) & 1u)) ok = false;
@@ -540,7 +543,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
                 }
                 __syncwarp();
             }
-            if (ok && !direct && here) as_store_ml(p, s.place, ROWS, row, ref == -INFINITY ? ref : ref - AO_LIFT, sum);
+            if (ok && !direct && here) as_store_ml(p, s.place, ROWS, row, ref, sum);
             mr += cnt;
             if (!ok) break;
             }

@@ -590,3 +590,26 @@ def test_generate_shared_ignores_what_pads_a_prompt():
         assert torch.equal(m.generate_shared(prefix, padded, 5, prompt_lengths=lens), want)
         with pytest.raises(ValueError, match="vocabulary"):
             m.generate_shared(prefix, padded, 5)
+
+
+@pytest.mark.parametrize("case", [(1, 3, 0, 90, 1, 4, 2, 16), (1, 5, 0, 300, 6, 8, 2, 64), (1, 40, 700, 90, 1, 32, 8, 64), (1, 140, 640, 40, 1, 4, 4, 32),
+                                  (1, 2, 200, 150, 100, 8, 2, 32)])
+@pytest.mark.parametrize("exponent", [20, 23, 24, 25, 26, 27, 28, 29, 40, 60])
+def test_scores_of_any_size(case, exponent):
+    """Scores beyond what 24 bits hold to a whole number: the largest take all weight, evenly where several keys are the same.  Keys are multiples of one
+    value, so scores are equal or apart by 2^-6 of the largest and more: every weight but theirs is zero, also in 64 bits."""
+    groups, per, shared, own, tps, nh, nkv, page = case
+    c, q, pos, slots, starts = batch(*case, seed=51)
+    g = torch.Generator(device="cuda").manual_seed(exponent)
+    q.zero_()
+    q.view(-1, nh, D)[:, :, 5] = 16384.0
+    keys = torch.randint(-64, 33, c.pool[0, 0, ..., 0].shape, device="cuda", generator=g)
+    keys[torch.rand(keys.shape, device="cuda", generator=g) < 0.02] = 33
+    c.pool[0, 0] = 0
+    c.pool[0, 0, ..., 5] = keys.half()
+    # scale: scores times log2(e) of up to 33 / 64 of 2^(exponent + 1)
+    scale = 2.0 ** (exponent - 19) * 0.6931471805599453
+    common = c.common(slots, starts)
+    ref = attention(c, 0, q, pos, slots, nh, scale)
+    for say in (dict(group_starts=starts, shared=common), {}):
+        close(c.attention(0, q, pos, slots, scale=scale, **say), ref, shared + own)

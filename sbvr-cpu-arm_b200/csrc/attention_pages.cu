@@ -99,9 +99,9 @@ __device__ __forceinline__ void ao_join_parts(AoJoin& j, const float* part, int 
         j.add(ml, v);
     }
 }
-__device__ __forceinline__ void ao_put(const AoParams& p, int token, int head, int d4, const AoJoin& j) {
+// `on`: the row attends to a key (else: zeros).  Scores that are all -inf leave l = 0 and o = 0: NaN, as zero over zero is.
+__device__ __forceinline__ void ao_put(const AoParams& p, int token, int head, int d4, const AoJoin& j, bool on) {
     const float inv = 1.0f / j.l;
-    const bool on = j.l > 0.0f || j.l != j.l;      // (a row without keys: zeros)
     const __half2 a = __floats2half2_rn(on ? j.o.x * inv : 0.0f, on ? j.o.y * inv : 0.0f), b = __floats2half2_rn(on ? j.o.z * inv : 0.0f, on ? j.o.w * inv : 0.0f);
     *reinterpret_cast<uint2*>(p.out + ((size_t)token * p.n_heads + head) * AO_D + d4 * 4) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
     extern __shared__ __align__(128) unsigned char ao_smem[];
     __shared__ float2 ml_s[AO_WARPS][16];          // a warp's m, l
     __shared__ __align__(16) float2 ml_c[16];      // the CTA's
+    __shared__ bool on_s[16];                      // rows that attend to a key
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int rps = p.tps * p.R, nrb = (rps + 15) / 16;
     const int unit = (int)blockIdx.x / nsplit, rank = (int)blockIdx.x - unit * nsplit;
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
         lim[h] = g + 8 * h < nrows ? ao_limit(p, __ldg(p.positions + (size_t)seq * p.tps + tok)) : 0;
         qrow[h] = p.q + ((size_t)seq * p.tps + tok) * p.q_pitch + ((size_t)kvh * p.R + (r - tok * p.R)) * AO_D;
     }
+    if (tid < 32 && t4 == 0) on_s[g] = lim[0] > 0, on_s[g + 8] = lim[1] > 0;
     const int most = __reduce_max_sync(0xffffffffu, max(lim[0], lim[1]));
     const int least = __reduce_min_sync(0xffffffffu, min(g < nrows ? lim[0] : INT_MAX, g + 8 < nrows ? lim[1] : INT_MAX));
     const int seen = __reduce_min_sync(0xffffffffu, min(lim[0] > 0 ? lim[0] : INT_MAX, lim[1] > 0 ? lim[1] : INT_MAX));      // (rows without keys come out as zeros)
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(AO_WARPS * 32) attention_own_kernel(const AoPa
         }
         if (from > 0) ao_join_parts(j, part, f.n, p.rows, prow + r, d4);
         const int row = row0 + r, tok = row / p.R;
-        ao_put(p, seq * p.tps + tok, kvh * p.R + (row - tok * p.R), d4, j);
+        ao_put(p, seq * p.tps + tok, kvh * p.R + (row - tok * p.R), d4, j, on_s[r]);
     }
     if (nsplit > 1) ao_cluster_sync();             // nobody leaves while its sums are read
 }
@@ -327,10 +329,11 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AoParams p, i
     if (tok >= p.tps) return;
     const int kvh = u % p.c.n_kv, seq = u / p.c.n_kv;
     const float* part = p.part + (size_t)block * nsplit * ao_place_floats(p.rows);
+    const bool on = ao_limit(p, __ldg(p.positions + (size_t)seq * p.tps + tok)) > 0;
     for (int d4 = threadIdx.x >> 5; d4 < 32; d4 += 8) {
         AoJoin j;
         ao_join_parts(j, part, nsplit, p.rows, row, d4);
-        ao_put(p, seq * p.tps + tok, kvh * p.R + (at_row - tok * p.R), d4, j);
+        ao_put(p, seq * p.tps + tok, kvh * p.R + (at_row - tok * p.R), d4, j, on);
     }
 }
 

@@ -206,7 +206,7 @@ __device__ __noinline__ void as_multiply_out(const AoParams& p, const AsSeg& s, 
             if (lane == 0) as_store_ml(p, s.place, rows, row, m, l * AO_LIFTED);
         } else {
             const float inv = 1.0f / l;
-            const bool on = l > 0.0f || l != l;
+            const bool on = end > 0;                             // (a prompt's rows: all of their keys are this piece's)
             const __half2 a = __floats2half2_rn(on ? o[0] * inv : 0.0f, on ? o[1] * inv : 0.0f), b = __floats2half2_rn(on ? o[2] * inv : 0.0f, on ? o[3] * inv : 0.0f);
             *reinterpret_cast<uint2*>(p.out + ((size_t)token * p.n_heads + head) * AO_D + lane * 4) =
                 make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(AsShape<NT>::THREADS, NT == 1 ? 2 : 1)
             aq_fence_after();
             const bool direct = s.place < 0;
             const float inv = 1.0f / sum;
-            const bool on = sum > 0.0f || sum != sum;
+            const bool on = lim > 0;                             // (scores that are all -inf: zero over zero)
             __half* dst = p.out + ((size_t)token * p.n_heads + head) * AO_D;
 #pragma unroll 1
             for (int c = 0; c < 4 && ok; ++c) {

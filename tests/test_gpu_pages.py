@@ -613,3 +613,30 @@ def test_scores_of_any_size(case, exponent):
     ref = attention(c, 0, q, pos, slots, nh, scale)
     for say in (dict(group_starts=starts, shared=common), {}):
         close(c.attention(0, q, pos, slots, scale=scale, **say), ref, shared + own)
+
+
+@pytest.mark.parametrize("case", [(1, 3, 0, 90, 1, 4, 2, 16), (1, 5, 0, 300, 6, 8, 2, 64), (1, 40, 700, 90, 1, 32, 8, 64), (1, 140, 640, 40, 1, 4, 4, 32),
+                                  (1, 2, 200, 150, 100, 8, 2, 32), (1, 60, 200, 150, 100, 8, 8, 32)])
+def test_scores_of_minus_infinity(case):
+    """Keys with infinities: no weight where other scores are finite, NaN where there is no other (zero over zero), zeros for a row without keys."""
+    groups, per, shared, own, tps, nh, nkv, page = case
+    c, q, pos, slots, starts = batch(*case, seed=61)
+    q.view(-1, nh, D)[:, :, 5] = 1.0
+    pos[tps if tps > 1 else 2] = -1                            # (a place without a token among others)
+    some, none = slots[0], slots[1]
+    for s, cut in ((some, 20), (none, None)):
+        own_pages = [int(p) for p in c.table[s] if p >= 0 and c.refs[p] == 1]
+        c.pool[0, 0, own_pages, ..., 5] = float("-inf")
+        if cut and int(c.lengths[s]) > shared + 1:             # its last token's key is finite
+            at = int(c.lengths[s]) - 1
+            c.pool[0, 0, int(c.table[s, at // page]), :, at % page] = 0.25
+    if shared:
+        c.pool[0, 0, c.table[slots[0], :shared // page].long(), ..., 5] = float("-inf")
+    ref = attention(c, 0, q, pos, slots, nh)
+    common = c.common(slots, starts)
+    for say in (dict(group_starts=starts, shared=common), {}):
+        out = c.attention(0, q, pos, slots, **say)
+        nan = torch.isnan(ref[0])
+        assert nan.any() and torch.equal(torch.isnan(out), nan)
+        close(out.masked_fill(nan, 0), tuple(x.masked_fill(nan, 0) for x in ref), shared + own)
+        assert not out[pos < 0].any()

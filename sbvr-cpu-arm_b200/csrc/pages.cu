@@ -128,10 +128,10 @@ constexpr int PG_POSITIONS = 8192, PG_SHARED = 2048;
 __global__ void __launch_bounds__(256) pages_positions_kernel(const PgCache c, const int* slots, const int* tokens, int each, int* positions, int tps) {
     pdl_launch_dependents();
     pdl_wait();
-    const int s = blockIdx.y, t = tokens ? tokens[s] : each;
+    const int s = blockIdx.x, t = tokens ? tokens[s] : each;
     const bool done = c.scratch[0] == 0;
     const int first = done ? c.lengths[pg_slot(slots, s)] - t : 0, end = done ? t : 0;
-    for (int j = blockIdx.x * 256 + threadIdx.x; j < tps; j += gridDim.x * 256) positions[(size_t)s * tps + j] = j < end ? first + j : -1;
+    for (int j = blockIdx.y * 256 + threadIdx.x; j < tps; j += gridDim.y * 256) positions[(size_t)s * tps + j] = j < end ? first + j : -1;
 }
 
 __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const PgCache c, const int* slots, const int* tokens, int each, int n,
@@ -590,11 +590,10 @@ int sbvr_pages_reserve(const sbvr_pages_t* cache, const int* slots, const int* t
     if (n < 1 || n > c.max_seqs || (!tokens && tokens_each < 0) || (positions && tokens_per_seq < 1)) return SBVR_ERR_BAD_ARG;
     if (positions && (long long)n * tokens_per_seq > INT_MAX / 2) return SBVR_ERR_UNSUPPORTED;
     const bool many = positions && (long long)n * tokens_per_seq > PG_POSITIONS;
-    if (many && n > 65535) return SBVR_ERR_UNSUPPORTED;
     SBVR_CUDA_TRY(launch_pdl(pages_reserve_kernel, dim3(1), dim3(PG_THREADS), seen_bytes(c) + (n <= PG_SHARED ? (2 * (size_t)n + 1) * 4 : 0), reinterpret_cast<cudaStream_t>(stream), c, slots, tokens,
                              tokens_each, n, many ? nullptr : positions, tokens_per_seq));
     if (many)
-        SBVR_CUDA_TRY(launch_pdl(pages_positions_kernel, dim3((unsigned)std::min((tokens_per_seq + 1023) / 1024, 64), (unsigned)n), dim3(256), 0,
+        SBVR_CUDA_TRY(launch_pdl(pages_positions_kernel, dim3((unsigned)n, (unsigned)std::min((tokens_per_seq + 1023) / 1024, 64)), dim3(256), 0,
                                  reinterpret_cast<cudaStream_t>(stream), c, slots, tokens, tokens_each, positions, tokens_per_seq));
     return SBVR_OK;
 }

@@ -640,3 +640,24 @@ def test_scores_of_minus_infinity(case):
         assert nan.any() and torch.equal(torch.isnan(out), nan)
         close(out.masked_fill(nan, 0), tuple(x.masked_fill(nan, 0) for x in ref), shared + own)
         assert not out[pos < 0].any()
+
+
+def test_a_token_for_each_of_65536_slots():
+    """The largest cache's slots all at once, few and many positions each."""
+    from models.pages import PagedCache
+    n = 65536
+    c = PagedCache(1, 1, n, page_size=16, max_seqs=n, max_pages=1)
+    assert torch.equal(c.reserve(None, 1, tokens_per_seq=1), torch.zeros(n, dtype=torch.int32, device="cuda"))
+    some = torch.arange(n, device="cuda", dtype=torch.int32) % 16
+    got = c.reserve(None, some, tokens_per_seq=17).view(n, 17)
+    want = 1 + torch.arange(17, device="cuda", dtype=torch.int32).expand(n, 17)
+    assert torch.equal(got, torch.where(want <= some[:, None], want, torch.full_like(want, -1)))
+    c.check()
+    assert torch.equal(c.lengths, 1 + some) and (c.refs == 1).all()
+    assert torch.equal(c.table.view(-1), torch.arange(n, device="cuda", dtype=torch.int32))
+    c.reserve(None, 16)
+    with pytest.raises(RuntimeError, match="beyond"):
+        c.check()
+    c.free(torch.arange(n, device="cuda", dtype=torch.int32))
+    assert not c.refs.any() and not c.lengths.any() and (c.table == -1).all()
+    c.check()

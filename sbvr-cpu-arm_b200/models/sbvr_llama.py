@@ -291,13 +291,14 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
     # ------------------------------------------------------------------ buffers
     def _act(self, tokens: int, rows_out: int) -> _Buffers:
         key = (tokens, rows_out)
-        b = self._bufs.get(key)
-        if b is not None:
-            return b
+        if key not in self._bufs:
+            self._bufs[key] = self._new_act(tokens, rows_out, self._nsplit(tokens))
+        return self._bufs[key]
+
+    def _new_act(self, tokens: int, rows_out: int, nsplit: int) -> _Buffers:
         c, dev = self.config, self.device
         f16 = dict(dtype=torch.float16, device=dev)
         H = c.hidden_size
-        nsplit = self._nsplit(tokens)
         b = _Buffers(
             tokens=tokens,
             ids=torch.zeros(tokens, dtype=torch.int32, device=dev),
@@ -313,7 +314,6 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
                                      device=dev) if nsplit > 1 else None))
         if self.tp_size > 1:
             b.extra["gathered"] = torch.empty((self.tp_size, rows_out, self.vocab_local), **f16)
-        self._bufs[key] = b
         return b
 
     def _nsplit(self, tokens: int) -> int:
@@ -544,8 +544,7 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
     def attach_pages(self, pages: int, page_size: int = 64, max_seqs: Optional[int] = None, max_pages: Optional[int] = None) -> PagedCache:
         """Gives the model a cache in pages for `generate_shared` (beside the dense one of `generate`, which may be built for few tokens)."""
         self._shared_graph = None
-        for key in [k for k in self._bufs if k[0] == "paged"]:
-            del self._bufs[key]
+        self._keep_paged()
         self.pages = PagedCache(self.config.num_hidden_layers, self.n_kv, pages, page_size, max_seqs or self.max_batch, max_pages,
                                 self.config.head_dim, self.device)
         return self.pages
@@ -554,16 +553,20 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
         key = ("paged", tokens, rows_out, seqs)
         b = self._bufs.get(key)
         if b is None:
-            plain = self._bufs.pop((tokens, rows_out), None)
-            b = self._act(tokens, rows_out)
-            del self._bufs[(tokens, rows_out)]
-            if plain is not None:
-                self._bufs[(tokens, rows_out)] = plain
+            b = self._new_act(tokens, rows_out, 1)     # (attention on pages brings scratch of its own)
             i32 = dict(dtype=torch.int32, device=self.device)
             b.extra["paged"] = {"slots": torch.arange(seqs, **i32), "starts": torch.tensor([0, seqs], **i32), "shared": torch.zeros(1, **i32),
                                 "q": torch.empty((tokens, self.n_heads * self.config.head_dim), dtype=torch.float16, device=self.device)}
             self._bufs[key] = b
         return b
+
+    def _keep_paged(self, *keys) -> None:
+        """Gives back activations in pages but those named and those of the captured step: texts' lengths differ from call to call."""
+        if self._shared_graph is not None:
+            B = self._shared_graph[0]
+            keys += (("paged", B, B, B),)
+        for key in [k for k in self._bufs if k[0] == "paged" and k not in keys]:
+            del self._bufs[key]
 
     def _checked_ids(self, ids: torch.Tensor, lens: Optional[List[int]] = None) -> torch.Tensor:
         """Token ids as the embedding reads them, int32 on the model's device.  With `lens`, row i of `ids` holds lens[i] tokens; the places behind
@@ -604,13 +607,18 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             raise ValueError(f"slots 0 .. {B - 1} of the cache hold sequences already")
         prefix, prompts = self._checked_ids(prefix_ids), self._checked_ids(prompt_ids, lens)
         out = torch.empty((B, max_new_tokens), dtype=torch.int32, device=self.device)
+        mine = (("paged", B, B, B), ("paged", B * P, B, B))
+        self._keep_paged(*mine)
         try:
             if L:                                      # the common beginning, once, in slot 0
                 b = self._act_paged(L, 1, 1)
                 b.ids.copy_(prefix)
                 b.positions.copy_(cache.reserve(b.extra["paged"]["slots"], L, tokens_per_seq=L))
                 b.extra["paged"]["shared"].zero_()
+                b.extra["last"] = None                 # (of one prompt as long as the text: the same set)
                 self._forward_rows(b, L, last_only=True)
+                del b
+                self._keep_paged(*mine)
                 if B > 1:
                     cache.fork([0] * (B - 1), list(range(1, B)))
             d = self._act_paged(B, B, B)

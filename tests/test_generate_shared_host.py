@@ -103,3 +103,37 @@ def test_what_a_step_runs_on_changes_and_its_graphs_go(monkeypatch):
         m.tp_group, m._graph, m._shared_graph = "group", "dense", (1, "in pages")
         assert m.enable_fused_allreduce() is not unavailable
         assert m._graph is None and m._shared_graph is None
+
+
+def _bytes(m):
+    held = [t for b in m._bufs.values() for t in list(vars(b).values()) + list(b.extra.get("paged", {}).values()) if isinstance(t, torch.Tensor)]
+    return sum(t.untyped_storage().nbytes() for t in held)
+
+
+def test_activations_of_earlier_calls_are_not_kept(monkeypatch):
+    """A prefix's activations are 12 KB a token of this model: they live for the call, a batch of prompts' until the next call, a captured step's with it."""
+    m = model(monkeypatch, Cache(pages=200, max_seqs=8, max_pages=100))
+    most = 0
+    for L, B, P in ((300, 3, 5), (301, 3, 6), (700, 2, 9), (16, 1, 16), (0, 8, 1), (1000, 3, 5)):
+        m.generate_shared(torch.zeros(L, dtype=torch.long), torch.zeros((B, P), dtype=torch.long), 2, use_graph=False)
+        assert set(m._bufs) == {("paged", B, B, B), ("paged", B * P, B, B)}
+        most = max(most, _bytes(m))
+    assert most < 60 * 20000
+    m._shared_graph = (2, None)
+    m._act_paged(2, 2, 2)
+    step = m._bufs["paged", 2, 2, 2]
+    for L, B, P in ((300, 3, 5), (2, 1, 2), (7, 2, 9), (9, 3, 1)):
+        m.generate_shared(torch.zeros(L, dtype=torch.long), torch.zeros((B, P), dtype=torch.long), 1, use_graph=False)
+        assert m._bufs["paged", 2, 2, 2] is step and len(m._bufs) <= 3
+    m._drop_graphs()
+    m.generate_shared(torch.zeros(9, dtype=torch.long), torch.zeros((3, 5), dtype=torch.long), 1, use_graph=False)
+    assert set(m._bufs) == {("paged", 3, 3, 3), ("paged", 15, 3, 3)}
+
+
+def test_activations_in_pages_have_no_scratch_of_the_dense_cache(monkeypatch):
+    m = model(monkeypatch, Cache())
+    dense = m._act(4, 4)
+    assert dense.att_scratch is not None                       # (a step of four tokens splits the dense cache's keys)
+    m.generate_shared(torch.zeros(9, dtype=torch.long), torch.zeros((4, 3), dtype=torch.long), 2, use_graph=False)
+    assert m._act(4, 4) is dense
+    assert all(b.att_scratch is None for key, b in m._bufs.items() if key[0] == "paged")

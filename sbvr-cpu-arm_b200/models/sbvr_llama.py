@@ -601,10 +601,14 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
             raise ValueError("every prompt needs at least one token, and no more than its row holds")
         whole = L // page
         need = [-(-(L + n + max_new_tokens - 1) // page) for n in lens]
-        if B > cache.max_seqs or max(need) > cache.max_pages or whole + sum(n - whole for n in need) > cache.pages:
+        need_all = whole + sum(n - whole for n in need)
+        if B > cache.max_seqs or max(need) > cache.max_pages or need_all > cache.pages:
             raise ValueError("sequences beyond the cache in pages that this model was given")
+        cache.check()                                  # what earlier calls could not do is not this one's
         if bool(cache.lengths[:B].any()):
             raise ValueError(f"slots 0 .. {B - 1} of the cache hold sequences already")
+        if need_all > int((cache.refs == 0).sum()):
+            raise ValueError("other slots hold too many of the cache's pages")
         prefix, prompts = self._checked_ids(prefix_ids), self._checked_ids(prompt_ids, lens)
         out = torch.empty((B, max_new_tokens), dtype=torch.int32, device=self.device)
         mine = (("paged", B, B, B), ("paged", B * P, B, B))

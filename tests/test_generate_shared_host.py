@@ -137,3 +137,26 @@ def test_activations_in_pages_have_no_scratch_of_the_dense_cache(monkeypatch):
     m.generate_shared(torch.zeros(9, dtype=torch.long), torch.zeros((4, 3), dtype=torch.long), 2, use_graph=False)
     assert m._act(4, 4) is dense
     assert all(b.att_scratch is None for key, b in m._bufs.items() if key[0] == "paged")
+
+
+def test_pages_that_other_slots_hold_are_not_counted_on(monkeypatch):
+    m = model(monkeypatch, Cache(pages=20, page_size=16, max_seqs=4, max_pages=20))
+    prefix, prompts = torch.zeros(40, dtype=torch.long), torch.zeros((2, 5), dtype=torch.long)
+    m.generate_shared(prefix, prompts, 4, use_graph=False)     # two pages in common, one more each
+    m.steps.clear()
+    m.pages.m.reserve([3], [16 * 17], 0)
+    with pytest.raises(ValueError, match="pages"):
+        m.generate_shared(prefix, prompts, 4, use_graph=False)
+    assert not m.steps and sum(m.pages.m.refs) == 17 and not any(m.pages.m.lengths[:3]) and not m.pages.m.status
+    m.pages.m.free([3]), m.pages.m.reserve([3], [16 * 16], 0)
+    assert m.generate_shared(prefix, prompts, 4, use_graph=False).shape == (2, 4)
+
+
+def test_what_earlier_calls_could_not_do_is_said_before_anything_is_run(monkeypatch):
+    m = model(monkeypatch, Cache())
+    prompts = torch.zeros((2, 5), dtype=torch.long)
+    m.pages.reserve([0], 10 ** 6)
+    with pytest.raises(RuntimeError, match="status 2"):
+        m.generate_shared(prompts[0], prompts, 4, use_graph=False)
+    assert not m.steps
+    assert m.generate_shared(prompts[0], prompts, 4, use_graph=False).shape == (2, 4)

@@ -661,3 +661,21 @@ def test_a_token_for_each_of_65536_slots():
     c.free(torch.arange(n, device="cuda", dtype=torch.int32))
     assert not c.refs.any() and not c.lengths.any() and (c.table == -1).all()
     c.check()
+
+
+def test_generate_shared_beside_other_sequences():
+    """Slots of others are left as they are; pages that they hold are not counted on."""
+    m = tiny()
+    c = m.attach_pages(20, 16, max_seqs=4)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    prefix = torch.randint(0, 1024, (40,), device="cuda", generator=g)
+    prompts = torch.randint(0, 1024, (2, 5), device="cuda", generator=g)
+    want = m.generate_shared(prefix, prompts, 4)
+    c.reserve([3], 16 * 16)
+    book = c.book.clone()
+    assert torch.equal(m.generate_shared(prefix, prompts, 4), want) and torch.equal(c.book, book)
+    c.reserve([3], 1)
+    with pytest.raises(ValueError, match="pages"):
+        m.generate_shared(prefix, prompts, 4)
+    c.free([3])
+    assert torch.equal(m.generate_shared(prefix, prompts, 4, use_graph=False), want)

@@ -29,6 +29,8 @@ class PagedCache:
     One call at a time: calls that may overlap on the GPU (other streams) have to be ordered by the caller.
     """
 
+    FORK_PAIRS = 1024                              # of one fork or copy, which does all of them at once
+
     def __init__(self, layers: int, n_kv: int, pages: int, page_size: int = 64, max_seqs: int = 64, max_pages: Optional[int] = None,
                  head_dim: int = 128, device="cuda"):
         if head_dim != 128:
@@ -96,7 +98,8 @@ class PagedCache:
         _lib.native.pages_free(self._at, self.device.index, self._slots(slots))
 
     def fork(self, src: Slots, dst: Slots) -> None:
-        """Slot dst[i] becomes what slot src[i] is, all at once: whole pages in common, the tokens of a part-filled last page copied."""
+        """Slot dst[i] becomes what slot src[i] is, all at once (at most FORK_PAIRS): whole pages in common, the tokens of a part-filled last page
+        copied."""
         _lib.native.pages_fork(self._at, self.device.index, self._slots(src, "src", True), self._slots(dst, "dst"), 1)
 
     def copy(self, src: Slots, dst: Slots) -> None:

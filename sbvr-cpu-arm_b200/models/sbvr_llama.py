@@ -623,8 +623,9 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
                 self._forward_rows(b, L, last_only=True)
                 del b
                 self._keep_paged(*mine)
-                if B > 1:
-                    cache.fork([0] * (B - 1), list(range(1, B)))
+                for first in range(1, B, PagedCache.FORK_PAIRS):
+                    children = list(range(first, min(B, first + PagedCache.FORK_PAIRS)))
+                    cache.fork([0] * len(children), children)
             d = self._act_paged(B, B, B)
             d.extra["paged"]["shared"].copy_(cache.common(d.extra["paged"]["slots"], d.extra["paged"]["starts"]))
             b = self._act_paged(B * P, B, B) if P > 1 else d

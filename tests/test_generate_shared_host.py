@@ -160,3 +160,12 @@ def test_what_earlier_calls_could_not_do_is_said_before_anything_is_run(monkeypa
         m.generate_shared(prompts[0], prompts, 4, use_graph=False)
     assert not m.steps
     assert m.generate_shared(prompts[0], prompts, 4, use_graph=False).shape == (2, 4)
+
+
+def test_more_prompts_than_a_fork_takes(monkeypatch):
+    n = 1100
+    m = model(monkeypatch, Cache(pages=n + 10, page_size=16, max_seqs=n, max_pages=3))
+    out = m.generate_shared(torch.zeros(17, dtype=torch.long), torch.zeros((n, 2), dtype=torch.long), 2, use_graph=False)
+    assert out.shape == (n, 2)
+    assert m.steps[1][1].view(n, 2).tolist() == [[17, 18]] * n and m.steps[2][1].tolist() == [19] * n
+    assert not m.pages.refs.any()

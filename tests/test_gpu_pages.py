@@ -679,3 +679,18 @@ def test_generate_shared_beside_other_sequences():
         m.generate_shared(prefix, prompts, 4)
     c.free([3])
     assert torch.equal(m.generate_shared(prefix, prompts, 4, use_graph=False), want)
+
+
+def test_generate_shared_for_more_prompts_than_a_fork_takes():
+    """1030 prompts, ten different ones in turn: the same prompt, the same tokens and logits (every row of a batch goes through the same kernels)."""
+    m = tiny()
+    c = m.attach_pages(1200, 16, max_seqs=1030, max_pages=4)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    prefix = torch.randint(0, 1024, (20,), device="cuda", generator=g)
+    ten = torch.randint(0, 1024, (10, 3), device="cuda", generator=g)
+    out = m.generate_shared(prefix, ten.repeat(103, 1), 3)
+    logits = m._bufs["paged", 1030, 1030, 1030].logits.view(103, 10, -1).double()
+    assert torch.equal(out, out[:10].repeat(103, 1))
+    assert ((logits - logits[0]).norm(dim=-1) < 1e-2 * logits.norm(dim=-1)).all()
+    assert (logits[0, 1:] - logits[0, :-1]).norm(dim=-1).min() > 1e-2 * logits[0].norm(dim=-1).max()
+    assert not c.refs.any()

@@ -694,3 +694,45 @@ def test_generate_shared_for_more_prompts_than_a_fork_takes():
     assert ((logits - logits[0]).norm(dim=-1) < 1e-2 * logits.norm(dim=-1)).all()
     assert (logits[0, 1:] - logits[0, :-1]).norm(dim=-1).min() > 1e-2 * logits[0].norm(dim=-1).max()
     assert not c.refs.any()
+
+
+@pytest.mark.parametrize("L,B,P,page,new", [(100, 5, 9, 16, 22), (33, 1, 1, 32, 4), (0, 3, 7, 16, 12), (200, 8, 40, 64, 40), (64, 4, 1, 64, 3), (5, 2, 70, 16, 9)])
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_steps_of_generate_shared_against_the_dense_cache(L, B, P, page, new, use_graph):
+    """The logits of several steps, across pages' ends, are those of the dense model on the whole sequence: prefix, prompt and the tokens so far (1e-2, the bound
+    of this model's outputs); the token is the dense one's where its lead is larger than two rows' worth of that."""
+    m = tiny()
+    m.attach_pages(100, page, max_seqs=8)
+    g = torch.Generator(device="cuda").manual_seed(L + P)
+    prefix = torch.randint(0, 1024, (L,), device="cuda", generator=g)
+    prompts = torch.randint(0, 1024, (B, P), device="cuda", generator=g)
+    lens = [P] + [1 + (5 * i) % P for i in range(1, B)]
+    for k in sorted({2, 3, new // 2, new - 1, new} - {0, 1}):
+        got = m.generate_shared(prefix, prompts, k, prompt_lengths=lens, use_graph=use_graph)
+        logits = m._bufs["paged", B, B, B].logits.double()
+        for i in range(B):
+            ids = torch.cat((prefix, prompts[i, :lens[i]], got[i, :-1].long()))[None]
+            want = m.forward(ids)[0, -1].double()
+            assert (logits[i] - want).norm() < 1e-2 * want.norm(), (k, i)
+            lead = want.topk(2).values
+            if lead[0] - lead[1] > 2 * 1e-2 * want.norm():
+                assert int(got[i, -1]) == int(want.argmax())
+            assert int(got[i, -1]) == int(m._bufs["paged", B, B, B].logits[i].argmax())
+
+
+def test_logits_of_padded_prompts():
+    """The pad ids of test_generate_shared_ignores_what_pads_a_prompt, seen in the logits of the last step: the same bits."""
+    m = tiny()
+    m.attach_pages(60, 16, max_seqs=8)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    prefix = torch.randint(0, 1024, (37,), device="cuda", generator=g)
+    prompts = torch.randint(0, 1024, (4, 9), device="cuda", generator=g)
+    lens, seen = [9, 1, 4, 8], []
+    for pad in (None, -1, -100, 2 ** 31 - 1):
+        padded = prompts.clone()
+        for i, n in enumerate(lens):
+            if pad is not None:
+                padded[i, n:] = pad
+        m.generate_shared(prefix, padded, 5, prompt_lengths=lens)
+        seen.append(m._bufs["paged", 4, 4, 4].logits.clone())
+    assert torch.isfinite(seen[0]).all() and all(torch.equal(s, seen[0]) for s in seen[1:])

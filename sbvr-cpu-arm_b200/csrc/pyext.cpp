@@ -371,6 +371,15 @@ PyObject* py_row_deq(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- a cache in pages (models/pages.py holds the tensors and the description of them) -----------------------------------------------
 // Every function begins (cache, device): the address of an sbvr_pages_t that the caller keeps, and the device of its memory.
+template <typename F>
+void launched(F call, const char* name) {          // without the interpreter's lock (nothing of Python's in `call`): a full stream holds a launch up
+    int rc;
+    {
+        ReleaseGil nogil;
+        rc = call();
+    }
+    check(rc, name);
+}
 struct Pages {
     const sbvr_pages_t* c;
     int dev;
@@ -429,8 +438,9 @@ PyObject* py_pages_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int tps = as_int(a[5]);
         if (tps < 0) fail(PyExc_ValueError, "tokens_per_seq must not be negative");
         if (tps) positions = at::empty({k * tps}, at::TensorOptions().dtype(at::kInt).device(p.device()));
-        check(sbvr_pages_reserve(p.c, ints(slots), ints(tokens), each ? as_int(a[4]) : 0, (int)k, tps ? positions.data_ptr<int>() : nullptr, tps, p.stream),
-              "sbvr_pages_reserve");
+        const int count = each ? as_int(a[4]) : 0;
+        launched([&] { return sbvr_pages_reserve(p.c, ints(slots), ints(tokens), count, (int)k, tps ? positions.data_ptr<int>() : nullptr, tps, p.stream); },
+                 "sbvr_pages_reserve");
         if (!tps) Py_RETURN_NONE;
         return THPVariable_Wrap(positions);
     });
@@ -440,7 +450,7 @@ PyObject* py_pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         Pages p(a, n, 3, "pages_free");
         at::Tensor slots = p.need(a[2], at::kInt, "slots");
-        check(sbvr_pages_free(p.c, ints(slots), (int)slots.numel(), p.stream), "sbvr_pages_free");
+        launched([&] { return sbvr_pages_free(p.c, ints(slots), (int)slots.numel(), p.stream); }, "sbvr_pages_free");
         Py_RETURN_NONE;
     });
 }
@@ -450,7 +460,8 @@ PyObject* py_pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Pages p(a, n, 5, "pages_fork");
         at::Tensor src = p.need(a[2], at::kInt, "src"), dst = p.need(a[3], at::kInt, "dst");
         if (src.numel() != dst.numel()) fail(PyExc_ValueError, "src and dst must be of one length");
-        check(sbvr_pages_fork(p.c, ints(src), ints(dst), (int)src.numel(), as_int(a[4]), p.stream), "sbvr_pages_fork");
+        const int share = as_int(a[4]);
+        launched([&] { return sbvr_pages_fork(p.c, ints(src), ints(dst), (int)src.numel(), share, p.stream); }, "sbvr_pages_fork");
         Py_RETURN_NONE;
     });
 }
@@ -458,7 +469,7 @@ PyObject* py_pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         Pages p(a, n, 2, "pages_compact");
-        check(sbvr_pages_compact(p.c, p.stream), "sbvr_pages_compact");
+        launched([&] { return sbvr_pages_compact(p.c, p.stream); }, "sbvr_pages_compact");
         Py_RETURN_NONE;
     });
 }
@@ -472,7 +483,8 @@ PyObject* py_pages_common(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t groups = starts.numel() - 1;
         if (groups < 1) fail(PyExc_ValueError, "group_starts must hold one number more than there are groups");
         at::Tensor out = at::empty({groups}, starts.options());
-        check(sbvr_pages_common(p.c, ints(slots), (int)k, ints(starts), (int)groups, out.data_ptr<int>(), p.stream), "sbvr_pages_common");
+        launched([&] { return sbvr_pages_common(p.c, ints(slots), (int)k, ints(starts), (int)groups, out.data_ptr<int>(), p.stream); },
+                 "sbvr_pages_common");
         return THPVariable_Wrap(out);
     });
 }
@@ -499,8 +511,11 @@ PyObject* py_pages_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (inv.numel() != D / 2) fail(PyExc_ValueError, "inv_freq must hold head_dim / 2 frequencies");
         if (!q.defined()) q = empty_half({T, nh * D}, p.device());
         else if (q.numel() != T * nh * D) fail(PyExc_ValueError, "q_out must be [tokens, n_heads * head_dim]");
-        check(sbvr_pages_rope_append_f16(p.c, as_int(a[2]), qkv.data_ptr(), ints(pos), inv.data_ptr<float>(), (float)scaling, ints(slots), (int)seqs, (int)tps,
-                                         (int)nh, q.data_ptr(), p.stream), "sbvr_pages_rope_append_f16");
+        const int layer = as_int(a[2]);
+        launched([&] {
+            return sbvr_pages_rope_append_f16(p.c, layer, qkv.data_ptr(), ints(pos), inv.data_ptr<float>(), (float)scaling, ints(slots), (int)seqs, (int)tps,
+                                              (int)nh, q.data_ptr(), p.stream);
+        }, "sbvr_pages_rope_append_f16");
         return THPVariable_Wrap(q);
     });
 }
@@ -531,9 +546,11 @@ PyObject* py_pages_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         check(sbvr_pages_attention_scratch_bytes(p.c, (int)seqs, (int)tps, (int)nh, (int)groups, &bytes), "sbvr_pages_attention_scratch_bytes");
         at::Tensor scratch;                        // of this call: its memory goes to later work of the same stream (or graph) only
         if (bytes) scratch = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(p.device()));
-        check(sbvr_pages_attention_f16(p.c, as_int(a[2]), q.data_ptr(), T > 1 ? q.stride(0) : nh * D, ints(slots), ints(pos), ints(starts), ints(shared), (int)groups,
-                                       out.data_ptr(), ptr(scratch), bytes, (int)seqs, (int)tps, (int)nh, (float)scale, p.stream),
-              "sbvr_pages_attention_f16");
+        const int layer = as_int(a[2]);
+        launched([&] {
+            return sbvr_pages_attention_f16(p.c, layer, q.data_ptr(), T > 1 ? q.stride(0) : nh * D, ints(slots), ints(pos), ints(starts), ints(shared), (int)groups,
+                                            out.data_ptr(), ptr(scratch), bytes, (int)seqs, (int)tps, (int)nh, (float)scale, p.stream);
+        }, "sbvr_pages_attention_f16");
         return THPVariable_Wrap(out);
     });
 }

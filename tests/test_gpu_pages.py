@@ -736,3 +736,34 @@ def test_logits_of_padded_prompts():
         m.generate_shared(prefix, padded, 5, prompt_lengths=lens)
         seen.append(m._bufs["paged", 4, 4, 4].logits.clone())
     assert torch.isfinite(seen[0]).all() and all(torch.equal(s, seen[0]) for s in seen[1:])
+
+
+def test_calls_that_wait_for_room_in_the_stream_let_other_threads_run():
+    """A stream takes about a thousand launches ahead of the GPU; a call behind them waits in the driver, without the interpreter's lock."""
+    import threading
+    import time
+    c, q, pos, slots, starts = batch(1, 3, 40, 9, 1, 4, 2, 16, seed=71)
+    sl, common, nobody = ints(slots), c.common(slots, starts), ints([3])
+    inv, qkv = torch.ones(64, device="cuda"), torch.zeros((3, 8 * D), dtype=torch.float16, device="cuda")
+    calls = [lambda: c.free(nobody), lambda: c.reserve(nobody, 0), lambda: c.fork(nobody, nobody), lambda: c.compact(), lambda: c.common(sl, starts),
+             lambda: c.rope_append(0, qkv, pos, inv, sl), lambda: c.attention(0, q, pos, sl)]
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        done = threading.Event()
+
+        def work():
+            for _ in range(1500):
+                call()
+            done.set()
+        torch.cuda._sleep(800_000_000)                         # about half a second
+        t = threading.Thread(target=work)
+        worst, last, begun = 0.0, time.perf_counter(), time.perf_counter()
+        t.start()
+        while not done.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            worst, last = max(worst, now - last), now
+        t.join()
+        assert last - begun > 0.2 and worst < 0.1, (calls.index(call), worst, last - begun)
+        torch.cuda.synchronize()

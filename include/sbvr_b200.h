@@ -399,8 +399,10 @@ SBVR_API int sbvr_ll_reduce_add_rmsnorm_digits_f16(const void* recv_local, const
 
 /* ---- a KV cache in pages ----------------------------------------------------------------------------------------
  * Sequences live in slots; a slot's tokens k * page .. lie in page table[slot][k] of every layer, and a page may belong to several slots that
- * begin with the same tokens.  All pointers are device memory of the caller's; one call at a time may use a cache (they change it, and its
- * scratch), calls on one stream are in order.  Device state decides what a call does (free pages, lengths), so it is found out on the device:
+ * begin with the same tokens.  All pointers are device memory of the caller's.  reserve, free, fork, compact and rope_append change a cache (and some
+ * use its scratch): no other call on it may run at the same time.  common and attention only read it (and may leave a bit in *status): they may overlap
+ * one another, each attention with scratch of its own.  Calls on one stream are in order.  Device state decides what a call does (free pages,
+ * lengths), so it is found out on the device:
  * what cannot be done leaves the cache as it was and a bit in *status, which stays until the caller clears it.  All calls are asynchronous and
  * may be captured.  No counterpart in the reference, whose cache is the Hugging Face one (models/sbvr_llama.py:330-336). */
 typedef struct sbvr_pages {
@@ -444,9 +446,12 @@ SBVR_API int sbvr_pages_rope_append_f16(const sbvr_pages_t* cache, int layer, co
                                         float attn_scaling, const int* slots, int seqs, int tokens_per_seq, int n_heads, void* q_out,
                                         sbvr_stream_t stream);
 /* out[token][head] = softmax(q . K^T * scale) . V over positions 0 .. positions[token] of the slot of sequence token / tokens_per_seq (none below 0:
- * zeros).  q rows q_pitch elements apart (a multiple of 8), out [seqs * tokens_per_seq][n_heads * 128], which must not overlap q; n_heads a multiple of n_kv; scale > 0.
- * groups > 0: sequences group_starts[g] .. group_starts[g + 1] - 1 hold their first shared[g] tokens (whole pages count) in the same pages, those of
- * the group's first sequence are read, once for all of them (sbvr_pages_common finds them); sequences in no group share nothing.  groups = 0: nothing is shared.
+ * zeros; all scores -inf: NaN).  q rows q_pitch elements apart (a multiple of 8), out [seqs * tokens_per_seq][n_heads * 128], which must not overlap q;
+ * n_heads a multiple of n_kv; scale > 0.  Scores and sums are fp32; a weight is rounded to fp16 once for its product with v (2^-11 of it).
+ * groups > 0: sequences group_starts[g] .. group_starts[g + 1] - 1 hold their first shared[g] tokens (whole pages count) in the same pages
+ * (sbvr_pages_common finds them): the call may read those of the group's first sequence once for all of them, or every sequence's own entries of the
+ * table, which it does from 64 rows on (tokens_per_seq * n_heads / n_kv) and where sharing can save little.  Both have to be right.  Sequences in no
+ * group share nothing.  groups = 0: nothing is shared.
  * scratch: sbvr_pages_attention_scratch_bytes(), 16-byte aligned, not used by another call at the same time. */
 SBVR_API int sbvr_pages_attention_scratch_bytes(const sbvr_pages_t* cache, int seqs, int tokens_per_seq, int n_heads, int groups, size_t* bytes);
 SBVR_API int sbvr_pages_attention_f16(const sbvr_pages_t* cache, int layer, const void* q, long long q_pitch, const int* slots,

@@ -26,7 +26,8 @@ class PagedCache:
     int32 [max_seqs]; `refs` int32 [pages], how many slots hold a page.  The last three and `status` lie in `book`, so that a copy of that tensor
     keeps who holds what (not what the pages hold).
 
-    One call at a time: calls that may overlap on the GPU (other streams) have to be ordered by the caller.
+    `reserve`, `free`, `fork`, `copy`, `compact` and `rope_append` change the cache: the caller orders them with every other call on it (other streams).
+    `attention` and `common` only read it and may overlap one another.
     """
 
     FORK_PAIRS = 1024                              # of one fork or copy, which does all of them at once
@@ -137,7 +138,9 @@ class PagedCache:
                   group_starts: Optional[torch.Tensor] = None, shared: Optional[torch.Tensor] = None,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of q [tokens, n_heads * 128] (rows may lie apart) over the slots' tokens 0 .. positions[token].  `group_starts` [groups
-        + 1] and `shared` [groups] (from `common`): sequences group_starts[g] .. of the batch hold their first shared[g] tokens in the same pages,
-        which are read once for all of them."""
+        + 1] and `shared` [groups] (from `common`): sequences group_starts[g] .. of the batch hold their first shared[g] tokens in the same pages, so
+        the first one's may be read once for all of them (they are for fewer than 64 rows per sequence, tokens times heads per KV head, where that
+        saves enough; else every sequence's own).  Scores and sums are fp32, weights are rounded to fp16 once for their product with V (2^-11 of each;
+        the dense cache's attention keeps 2^-22 and more).  A row whose scores are all -inf is NaN, one at a position below 0 zeros."""
         return _lib.native.pages_attention(self._at, self.device.index, layer, q, positions, None if slots is None else self._slots(slots, twice=True),
                                            self.max_seqs, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, group_starts, shared, out)

@@ -380,7 +380,7 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
                 norm_linear(layer.qkv_proj, delta, layer.input_layernorm_weight, b.qkv)
             att_scratch = None if b.att_scratch is None else b.att_scratch.data_ptr()
             paged = b.extra.get("paged")
-            if paged is not None:                          # the cache in pages: what the sequences share is read once for all of them
+            if paged is not None:                          # the cache in pages: a step reads what the sequences share once for all of them
                 q = self.pages.rope_append(li, b.qkv, b.positions, self.inv_freq, paged["slots"], float(self.attention_scaling), q_out=paged["q"])
                 self.pages.attention(li, q, b.positions, paged["slots"], scale, paged["starts"], paged["shared"], out=b.ao)
             elif tokens_per_seq == 1 and self.fuse_glue:     # decode: rotary embedding and cache append inside attention

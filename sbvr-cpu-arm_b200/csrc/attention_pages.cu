@@ -354,7 +354,7 @@ static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int grou
     if (r.prompt) {
         r.rows = 128;
         r.blocks = (int)(seqs * c.n_kv * ((rps + r.rows - 1) / r.rows));
-        r.ctas = r.rows == 128 ? 2 * sm_count : sm_count;
+        r.ctas = 2 * sm_count;
         r.nsplit = std::max(1, std::min(64, r.ctas / r.blocks));
         r.places = r.nsplit > 1 ? (size_t)r.blocks * r.nsplit : 0;
     } else {

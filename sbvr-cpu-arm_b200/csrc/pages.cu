@@ -19,7 +19,6 @@ constexpr int PG_PER = 16;                         // pages a thread looks at in
 
 struct PgScan {                                    // exclusive prefix sums over the block's threads
     int warp[PG_THREADS / 32];
-    int total;
 };
 __device__ __forceinline__ int pg_scan(PgScan& s, int v, int* total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;

@@ -358,9 +358,12 @@ static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int grou
         r.nsplit = std::max(1, std::min(64, r.ctas / r.blocks));
         r.places = r.nsplit > 1 ? (size_t)r.blocks * r.nsplit : 0;
     } else {
-        // What sharing can save at most: reading what the slots can hold once per group instead of once per sequence.  Below 2 MB the second kernel alone is
-        // the faster form: it reads that in the time that the first takes to begin.
-        r.shared = groups > 0 && (long long)(seqs - groups) * c.max_pages * c.page * c.n_kv * (4 * AO_D) > (2 << 20);
+        // What sharing can save at most: reading what the slots can hold once per group instead of once per sequence (what they do hold, the device knows).
+        // The first kernel costs 9 us, in which the second reads the same keys again, most of them from L2.  With it and without, 8 KV heads, one token:
+        // 8 sequences on 1024 tokens (29 MB) 16.6 and 10.4 us, 16 on 1024 (64) 17.1, 15.6, 4 on 8192 (97) 27.4, 25.8, 16 on 2048 (124) 18.8, 24.9, 64 on
+        // 1024 (268) 25.4, 36.2; 2 KV heads, 4 on 32 768 (96) 37.4, 42.3; 8 tokens each, 16 on 1024 28.5, 28.5, on 2048 31.1, 47.4.  On the wrong side of
+        // the line: 128 on 256 (159) 31.5, 23.7; and few tokens in slots that could hold many, 4 of 2 KV heads on 256 15.0, 5.4.
+        r.shared = groups > 0 && (long long)(seqs - groups) * c.max_pages * c.page * c.n_kv * (4 * AO_D) > (100 << 20);
         if (r.shared) {
             r.rows = seqs * rps > 128LL * groups ? 256 : 128;
             r.per_block = r.rows / (int)rps;

@@ -767,3 +767,47 @@ def test_calls_that_wait_for_room_in_the_stream_let_other_threads_run():
         t.join()
         assert last - begun > 0.2 and worst < 0.1, (calls.index(call), worst, last - begun)
         torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ when the shared pages are read in common
+def wide_batch(*case, **kw):
+    """The same batch in a cache whose table could hold far more than it does: what sharing can save is counted by what slots can hold."""
+    from models.pages import PagedCache
+    c, *rest = narrow_batch(*case, **kw)
+    groups, per, _, _, _, _, nkv, page = case
+    width = max(c.max_pages, (128 << 20) // (max(1, groups * (per - 1)) * page * nkv * 512) + 1)
+    w = PagedCache(c.layers, c.n_kv, c.pages, page_size=page, max_seqs=c.max_seqs, max_pages=width)
+    w.pool.copy_(c.pool), w.table[:, :c.max_pages].copy_(c.table), w.lengths.copy_(c.lengths), w.refs.copy_(c.refs)
+    return (w, *rest)
+
+
+narrow_batch = batch
+FEW = [case for case in CASES if case[1] > 1 and case[4] * case[5] // case[6] < 64]
+
+
+@pytest.mark.parametrize("again", [lambda case=case: test_attention(case) for case in FEW] +
+                         [lambda a=a: test_growing_scores(tps=1, step=a) for a in (0.02, 0.7, 9.0)] +
+                         [lambda a=a: test_what_lies_behind_a_sequence_does_not_matter(a) for a in ((1, 4, 200, 30, 6, 8, 2, 16), (2, 9, 640, 20, 1, 8, 2, 128))] +
+                         [lambda a=a: test_values_that_are_not_finite_reach_the_tokens_that_see_them(tps=a, groups=True) for a in (1, 5, 6)] +
+                         [lambda a=a: test_entries_that_name_no_page(entry=-1, case=a) for a in ((1, 5, 200, 20, 1, 8, 2, 16), (1, 4, 300, 40, 6, 8, 2, 16))] +
+                         [lambda a=a: test_scores_of_any_size(exponent=a, case=(1, 5, 0, 300, 6, 8, 2, 64)) for a in (23, 27, 40)] +
+                         [lambda a=a: test_scores_of_any_size(exponent=a, case=(1, 6, 200, 300, 6, 8, 2, 64)) for a in (23, 26, 27, 28, 40)] +
+                         [lambda: test_scores_of_minus_infinity((1, 7, 300, 150, 3, 8, 2, 32)), lambda: test_rows_apart_and_scales(),
+                          lambda: test_any_batch_order_and_groups(), lambda: test_many_groups(), lambda: test_a_far_layer()])
+def test_small_batches_on_wide_tables(monkeypatch, again):
+    """Shared pages of any size, read in common."""
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "batch", wide_batch)
+    again()
+
+
+@pytest.mark.parametrize("case,launches", [((1, 4, 256, 40, 1, 4, 2, 16), 1), ((1, 8, 1024, 40, 1, 32, 8, 64), 1), ((1, 16, 1024, 40, 1, 32, 8, 64), 1),
+                                           ((1, 16, 2048, 40, 1, 32, 8, 64), 2), ((1, 64, 1024, 40, 1, 32, 8, 64), 2), ((16, 1, 2048, 40, 1, 32, 8, 64), 1),
+                                           ((1, 16, 2048, 40, 15, 32, 8, 64), 2)])
+def test_pages_are_read_in_common_where_that_pays(case, launches):
+    from launched import kernels
+    c, q, pos, slots, starts = batch(*case, seed=81)
+    common, sl = c.common(slots, starts), ints(slots)
+    names = kernels(lambda: c.attention(0, q, pos, sl, group_starts=starts, shared=common))
+    assert len(names) == launches and "attention_own_kernel" in names[-1] and (launches == 1 or "attention_shared_kernel" in names[0])
+    assert len(kernels(lambda: c.attention(0, q, pos, sl))) == 1

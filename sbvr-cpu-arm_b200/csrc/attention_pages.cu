@@ -350,6 +350,10 @@ struct AoPlan {
 static AoPlan ao_plan(const PgCache& c, int seqs, int tps, int n_heads, int groups, int sm_count) {
     AoPlan r = {};
     const long long rps = (long long)tps * (n_heads / c.n_kv);
+    // Rows of a block that share their keys, or a sequence's own 16 at a time?  8 KV heads of 4 query heads, 8, 12, 16, 20, 24 tokens each (32 to 96 rows),
+    // us as prompts / as few rows.  64 sequences, up to 2000 keys, none shared: 63, 68, 70, 72, 73 / 82, 110, 140, 171, 200.  8 such: 25, 26, 27, 28, 28 /
+    // 26, 39, 41, 43, 44.  One on 8000: 35, 37, 38, 39, 39 / 20, 26, 28, 43, 43.  64 on 8000 shared: 232, 267, 281, 294, 296 / 131, 202, 233, 339, 415.
+    // The lines lie between 32 and 80 rows.
     r.prompt = rps >= 64;
     if (r.prompt) {
         r.rows = 128;

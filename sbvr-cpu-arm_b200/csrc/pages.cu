@@ -381,8 +381,10 @@ __global__ void __launch_bounds__(256) pages_move_kernel(const PgCache c, int li
         }
     }
     const int planes = 2 * c.layers;
-    // a unit: some heads of one plane of one page; all heads where there are units enough for the grid
-    const int parts = (long long)count * planes >= 4 * (int)gridDim.x ? 1 : c.n_kv;
+    // A unit: one head of one plane of one page, or all heads, where planes make half the grid.  A fork's us by heads / by all, 8 heads: 64 planes of 250
+    // tokens 15.6 / 23.6, 256 of 120 21.7 / 25.0, 400 of 60 28.3 / 30.0; 448 of 15 19.5 / 12.7, 448 of 40 19.9 / 17.5, 960 of 40 30.8 / 23.9, 4032 of
+    // 40 96 / 74.  On the wrong side of the line: 512 of 120 36.0 / 39.8.
+    const int parts = (long long)count * planes * 2 >= (int)gridDim.x ? 1 : c.n_kv;
     const int heads = c.n_kv / parts;
     const long long units = (long long)count * planes * parts;
     for (long long u = blockIdx.x; u < units; u += gridDim.x) {

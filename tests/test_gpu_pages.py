@@ -811,3 +811,18 @@ def test_pages_are_read_in_common_where_that_pays(case, launches):
     names = kernels(lambda: c.attention(0, q, pos, sl, group_starts=starts, shared=common))
     assert len(names) == launches and "attention_own_kernel" in names[-1] and (launches == 1 or "attention_shared_kernel" in names[0])
     assert len(kernels(lambda: c.attention(0, q, pos, sl))) == 1
+
+
+@pytest.mark.parametrize("kids", [1, 4, 6, 7, 15])
+@pytest.mark.parametrize("share", [True, False])
+def test_copies_by_heads_and_by_planes(kids, share):
+    """64 to 2880 planes of pages to copy, three heads each: fewer than half the grid go head by head."""
+    c, m = make(layers=32, n_kv=3, pages=2 + 3 * (kids + 1), max_seqs=kids + 1, seed=kids)
+    c.reserve([0], 39), m.reserve([0], [39], 0)
+    (c.fork if share else c.copy)([0] * kids, list(range(1, kids + 1)))
+    m.fork([0] * kids, list(range(1, kids + 1)), share)
+    same(c, m)
+    gone = list(range(0, kids, 2))
+    c.free(gone), m.free(gone)
+    c.compact(), m.compact()
+    same(c, m)

@@ -18,8 +18,9 @@ namespace sbvr {
 // ---------------------------------------------------------------------------------------------
 // A sequence's own keys.  A cluster of `nsplit` CTAs per (sequence, KV head, 16 rows); every warp takes sixteen keys at a time, a running maximum
 // and sums of its own: no barrier until the end, when the warps' and the CTAs' parts are joined through (distributed) shared memory.  mma.sync: sixteen rows
-// at most share a key, so bytes and latencies bound it, not the products.  Two stages of sixteen keys per warp, 64 KB, three CTAs per SM; 16 x 4000 keys of 8 KV
-// heads (averages 2000) 44 us = 5.0 TB/s, 64 x 300 13 us; with three stages 40 and 15, with two warps per CTA 79 and 16.
+// at most share a key, so bytes and latencies bound it, not the products.  Two stages of sixteen keys per warp, 64 KB, three CTAs per SM: 16
+// sequences of up to 4000 keys, 8 KV heads (3393 on average, 222 MB) 39.5 us = 5.6 TB/s, 64 of up to 300 (154, 40 MB) 13.5 us = 3.0 TB/s, in a graph of
+// calls.  In a loop of calls 44 and 13, with three stages 40 and 15, with two warps per CTA 79 and 16.
 // ---------------------------------------------------------------------------------------------
 constexpr int AO_STAGES = 2, AO_KEYS = 16, AO_WARPS = 4, AO_PITCH = AO_D + 4;
 constexpr int AO_HALF_STAGE = AO_KEYS * AO_D * 2;                            // bytes of K or V of sixteen keys

@@ -20,10 +20,11 @@
 // uneven lengths leave less idle (8 x 300 tokens on 4001: 137 us; an earlier form 151, with 256 rows 164).  Every wait is bounded; a CTA in which one runs out, or among whose keys values are not finite that only
 // some rows attend to, multiplies its rows out without the tensor cores.
 //
-// What bounds it.  Few rows: bytes (32 KB a tile, 6.5 TB/s), behind 5 us of prologue (pieces, queries, the first keys) and 2 of sums.  Many rows: the chain from
-// scores to weights to outputs of a tile, about 1900 cycles for 256 rows, in which the tensor pipe works 1280 (768 for S, whose 64 columns read the queries
-// from shared memory again for each tile, 512 for O) and the units for exponentials 1024.  Without exponentials a launch takes as long, with an
-// eighth of the MMAs a tenth less.  Tried without gain: a polynomial for some exponentials, two warps per 32 rows, a warp each for the MMAs of S and of O.
+// What bounds it.  Few rows: bytes behind a prologue (pieces, queries, the first keys) and sums: 64 sequences of 4 heads, 16 on 8000 keys each, 132 MB, 36 us
+// alone and cold where the bytes need 20.  Many rows: the chain from scores to weights to outputs of a tile, 2260 cycles for 256 rows (128 sequences of 4 heads
+// on 65536 keys: 250 000 active cycles of an SM, 110.7 tiles), in which the tensor pipe counts 1024 as active (45 %) and the units for exponentials 1070 (47 %).
+// Without exponentials a launch takes as long, with an eighth of the MMAs a tenth less.  Tried without gain: a polynomial for some exponentials, two warps per
+// 32 rows, a warp each for the MMAs of S and of O.
 #include <cuda.h>
 
 #include <climits>

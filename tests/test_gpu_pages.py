@@ -826,3 +826,9 @@ def test_copies_by_heads_and_by_planes(kids, share):
     c.free(gone), m.free(gone)
     c.compact(), m.compact()
     same(c, m)
+
+
+@pytest.mark.parametrize("exponent", [23, 27, 40])
+def test_scores_of_any_size_in_whole_blocks(exponent):
+    """Prompts of so many sequences that a CTA has all keys of its rows and writes the output itself."""
+    test_scores_of_any_size((1, 60, 200, 150, 100, 8, 8, 32), exponent)

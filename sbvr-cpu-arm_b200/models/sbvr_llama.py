@@ -571,7 +571,7 @@ class SBVRLlamaForCausalLM(torch.nn.Module):
     def _checked_ids(self, ids: torch.Tensor, lens: Optional[List[int]] = None) -> torch.Tensor:
         """Token ids as the embedding reads them, int32 on the model's device.  With `lens`, row i of `ids` holds lens[i] tokens; the places behind
         them may hold anything (-1, a pad id) and become 0.  Every token has to be a row of the table: the kernel does not look.  Waits for the GPU."""
-        ids = ids.to(self.device)
+        ids = ids.to(self.device, torch.int64)         # (a byte is not compared with a large vocabulary)
         if lens is not None:
             held = torch.arange(ids.shape[1], device=self.device) < torch.tensor(lens, device=self.device)[:, None]
             ids = torch.where(held, ids, torch.zeros_like(ids))

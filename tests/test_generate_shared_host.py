@@ -169,3 +169,11 @@ def test_more_prompts_than_a_fork_takes(monkeypatch):
     assert out.shape == (n, 2)
     assert m.steps[1][1].view(n, 2).tolist() == [[17, 18]] * n and m.steps[2][1].tolist() == [19] * n
     assert not m.pages.refs.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_ids_of_any_whole_type(monkeypatch, dtype):
+    m = model(monkeypatch, Cache())
+    prompts = torch.arange(8, dtype=dtype).view(2, 4)
+    m.generate_shared(torch.arange(20, dtype=dtype), prompts, 2, prompt_lengths=[4, 2], use_graph=False)
+    assert m.steps[0][0].tolist() == list(range(20)) and m.steps[1][0].tolist() == [0, 1, 2, 3, 4, 5, 0, 0]

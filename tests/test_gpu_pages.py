@@ -756,7 +756,7 @@ def test_calls_that_wait_for_room_in_the_stream_let_other_threads_run():
             for _ in range(1500):
                 call()
             done.set()
-        torch.cuda._sleep(800_000_000)                         # about half a second
+        torch.cuda._sleep(1_200_000_000)                       # 0.6 s
         t = threading.Thread(target=work)
         worst, last, begun = 0.0, time.perf_counter(), time.perf_counter()
         t.start()
@@ -765,7 +765,7 @@ def test_calls_that_wait_for_room_in_the_stream_let_other_threads_run():
             now = time.perf_counter()
             worst, last = max(worst, now - last), now
         t.join()
-        assert last - begun > 0.2 and worst < 0.1, (calls.index(call), worst, last - begun)
+        assert last - begun > 0.3 and worst < 0.25, (calls.index(call), worst, last - begun)
         torch.cuda.synchronize()
 
 
